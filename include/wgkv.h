@@ -490,6 +490,67 @@ WGKV_API int wgkv_paged_decode_noalloc(const uint16_t* q, const uint16_t* k_cach
                                        int num_kv_heads, int head_dim, float softmax_scale, uint16_t* out, int* err,
                                        void* stream);
 
+/* ---- KV cache held in 4 bits ----------------------------------------------- */
+/*
+ * A paged cache of 4-bit codes (no reference counterpart: the reference's pool is bf16).  A value is
+ * scale * code + minimum, code in 0..15, with a bf16 (minimum, scale) pair for each `group` consecutive
+ * dimensions of one token's K or V row; group in {32, 64, 128}, at most head_dim, head_dim in {64, 128}.
+ * For a group with minimum m and maximum M, all steps in fp32:
+ *   scale = bf16((M - m) * (1/15)), 0 below 2^-126;
+ *   code  = floor(min((v - m) * (1 / scale) + (1/2 + 2^-12), 15.5)), 0 where scale is 0.
+ * A row (of K or of V) that holds a NaN or an infinity, or a group whose M - m is not finite, reads back
+ * as NaN throughout.
+ *   cache (num_pages, page_size, wgkv_kv4_row_bytes(head_dim, group)) uint8, 16-byte aligned: a page is
+ *   page_size / 16 records of 16 tokens (layout in csrc/kv4.cuh); no two tokens share a byte.
+ * A token costs head_dim + 8 * head_dim / group bytes, K and V together (bf16: 4 * head_dim).
+ * Returns WGKV_EINVAL for an unsupported pair.
+ */
+WGKV_API int wgkv_kv4_row_bytes(int head_dim, int group);
+
+/*
+ * Quantises rows as it writes them: row r of (b, h), r < min(counts[b, h], rows) (all `rows` when counts
+ * is NULL), goes to logical position start[b, h] + r of the pages block_table[b, h, :].  Nothing else of
+ * the cache is touched.  A row whose position lies outside the table's table_width pages is dropped and
+ * flags WGKV_ERR_HEAD_CAPACITY; one whose page id is not in [0, num_pages) is dropped and flags
+ * WGKV_ERR_BAD_PAGE.  Two rows must not name the same place in one call.
+ *   k, v (B, Hk, rows, D) bf16, element strides (sb, sh, st); start, counts (B, Hk) int32
+ *   block_table (B, Hk, table_width) int32, rows table_stride elements apart
+ * Constraints: page_size % 16 == 0; table_width * page_size < 2^31; B * Hk <= 65535.
+ */
+WGKV_API int wgkv_kv4_append(const uint16_t* k, int64_t k_sb, int64_t k_sh, int64_t k_st, const uint16_t* v,
+                             int64_t v_sb, int64_t v_sh, int64_t v_st, int batch, int kv_heads, int rows,
+                             int head_dim, int group, uint8_t* cache, int64_t num_pages, int page_size,
+                             const int32_t* start, const int32_t* counts, const int32_t* block_table,
+                             int64_t table_stride, int table_width, int* err, void* stream);
+
+/*
+ * Reads rows back: out_k / out_v (B, Hk, rows, D) bf16, contiguous and 16-byte aligned; row i of (b, h) is
+ * bf16(scale * code + minimum) of position start[b, h] + i (start NULL: 0) for i < min(counts[b, h],
+ * rows), zero behind it.  Positions and page ids out of range read as zero and flag the same errors.
+ */
+WGKV_API int wgkv_kv4_read(const uint8_t* cache, int64_t num_pages, int page_size, int head_dim, int group,
+                           const int32_t* start, const int32_t* counts, const int32_t* block_table,
+                           int64_t table_stride, int table_width, int batch, int kv_heads, int rows,
+                           uint16_t* out_k, uint16_t* out_v, int* err, void* stream);
+
+/*
+ * wgkv_paged_decode over a 4-bit cache: same q, out, cache_seqlens and block_table, the K and V values
+ * those that the cache stands for (unrounded).  A length past the table's pages flags
+ * WGKV_ERR_HEAD_CAPACITY and is cut there; a page id outside [0, num_pages) flags WGKV_ERR_BAD_PAGE and
+ * leaves that head's output undefined.  A head of length 0 (or below) yields zeros.  All sums and softmax
+ * statistics are fp32; the probabilities, times V's scale, are rounded to fp16 before the PV product.
+ * Constraints: (head_dim, group) as above; page_size % 16 == 0; Hq % Hk == 0; Hq / Hk <= 16;
+ * B * Hk <= 4096; B * Hk * table_width * page_size / 16 < 2^31; 16-byte aligned q, out and cache.
+ * workspace: wgkv_paged_decode_kv4_workspace_size() bytes, its first B*Hk*4 bytes zero before the first
+ * call (the kernel leaves them zero); calls sharing a workspace must be stream-ordered.
+ */
+WGKV_API size_t wgkv_paged_decode_kv4_workspace_size(int batch, int num_q_heads, int num_kv_heads, int head_dim);
+WGKV_API int wgkv_paged_decode_kv4(const uint16_t* q, const uint8_t* cache, int64_t num_pages, int page_size,
+                                   int group, const int32_t* cache_seqlens, const int32_t* block_table,
+                                   int64_t table_stride, int table_width, int batch, int num_q_heads,
+                                   int num_kv_heads, int head_dim, float softmax_scale, uint16_t* out,
+                                   void* workspace, size_t workspace_bytes, int* err, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

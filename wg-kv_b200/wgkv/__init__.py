@@ -14,6 +14,7 @@ from .decode import (  # noqa: F401
 from .gate import GatingPredictor, GatingRMSNorm, load_gate_checkpoint  # noqa: F401
 from .graph import DecodeGraph  # noqa: F401
 from .indices import generate_sparse_indices, sparse_indices_into  # noqa: F401
+from .kv4 import kv4_alloc, kv4_append, kv4_read, kv4_row_bytes, paged_decode_kv4  # noqa: F401
 from .layers import (  # noqa: F401
     decode_wrapper,
     migrate_local_kv_to_global,
@@ -28,7 +29,7 @@ from .layers import (  # noqa: F401
 )
 from .pool import RING_ON_DEVICE, WgkvPool, advance_host_ring, init_pool, ring_to_device  # noqa: F401
 from .prefill import sparse_attn_func, sparse_attn_func_pooled, sparse_attn_func_wrapper  # noqa: F401
-from . import ops  # noqa: F401  (torch.ops.wgkv.paged_decode, torch.ops.wgkv.sparse_attn)
+from . import ops  # noqa: F401  (torch.ops.wgkv.*)
 from .runtime import check_errors  # noqa: F401
 from .tp import KVHeadParallelAttention, shard_gate, shard_o_proj  # noqa: F401
 
