@@ -1,123 +1,602 @@
-// Ragged paged decode attention over a 4-bit KV cache (format: kv4.cuh).
+// Ragged paged decode attention over a 4-bit KV cache (format: kv4.cuh), sm_100a.
+//
+// With K = s_k c + m_k and V = s_v c + m_v per group of dimensions (c the codes, s and m the group's scale
+// and minimum), for every token t and query head h
+//   x_th = scale (sum_g s_k[t,g] (q_hg . c_tg) + m_k[t,g] (1 . q_hg)),
+//   out_h = (sum_t p_th s_v[t,g] c_t + sum_t p_th m_v[t,g]) / sum_t p_th,   p = 2^(x - reference),
+// so the matrix products run on the codes themselves and no value is ever expanded:
+//
+// * Tokens are the M side of both products (mma.m16n8k16, fp16 in, fp32 accumulate): S^T = C_k Q^T and
+//   O^T = C_v^T P^T with 8 query heads as N.  Up to 8 query heads per KV head take 16 instructions per 16
+//   tokens at D = 128, half of what heads on the M side (16 rows, mostly padding) would.
+// * A code is an fp16 operand without conversion: masked out of its word it is the subnormal code * 2^-24
+//   (bits 0-3) or code * 2^-20 (bits 4-7), which the tensor cores multiply exactly.  The factors are
+//   undone on q (odd k-steps carry q / 16) and on the output (odd m-tiles).  5 integer operations unpack
+//   8 codes.
+// * q enters as fp16 times a power of two per head that puts its largest element in [2^14, 2^15): exact
+//   down to 2^-24 of it, 2^-36 of it absolute below.
+// * The weights p s_v are rounded to fp16 (11 bits).  The reference 2^r of p is a running maximum over
+//   x + exponent(s_v), not over x, so that the weights, not the probabilities, are near 1 however V's
+//   scale differs between tokens; it moves only when a weight would pass 2^9.  Exponents below -40 count
+//   as -40.  Sums of p and p m_v stay fp32.
+// * S^T's accumulators hold a token per lane row, P^T's fragment a head per lane row: movmatrix turns the
+//   packed weights, one per 8x8 block.
+//
+// Work is cut as in paged_decode.cu: the 16-token records of all heads laid end to end, equal segments per
+// CTA, one producer warp that copies whole records (cp.async.bulk, page ids loaded a step ahead) into a
+// ring of stages, consumer warps with up to kNB records each per stage; a head cut over CTAs is merged by
+// the last one to finish it (self-resetting counter, fixed order of summation).
 #include "kv4.cuh"
 #include "runtime.h"
 
 namespace wgkv {
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kTile = 64;    // tokens per tile
+constexpr int kNCW = 7;                      // consumer warps; with the producer 8: 128 registers a thread at 2 CTAs per SM
+constexpr int kNB = 2;                       // records per consumer warp and stage
+constexpr int kStageRecs = kNCW * kNB;
+constexpr int kThreads = 32 * (kNCW + 1);
+constexpr int kMaxStages = 8;
+constexpr int kMaxBH = 4096;
 constexpr int kMaxG = 16;
+// CTAs per SM: the accumulators of two head tiles need the registers of the whole SM
+constexpr int ctas_per_sm(int head_tiles) { return head_tiles == 1 ? 2 : 1; }
 
 struct Kv4DecodeParams {
   Kv4Pages c;
   const uint16_t* q;
   uint16_t* out;
   const int32_t* seqlens;
-  int G;
+  int BH, G, stages;
   float scale_log2;
+  float* part;    // partial results: (BH + CTAs) x G x (D + 2)
+  int* counters;  // per head
 };
 
-// One CTA per (batch, kv head): tiles of 64 tokens are expanded to fp32 in shared memory, scores by
-// dot products, one running maximum and sum per query head; a thread owns one output dimension of every
-// query head.
-template <int D, int NG>
-__global__ void __launch_bounds__(kThreads) kv4_decode_kernel(Kv4DecodeParams p) {
-  extern __shared__ float sm[];
-  float* ks = sm;                     // [kTile][D + 1]
-  float* vs = ks + kTile * (D + 1);   // [kTile][D]
-  float* qs = vs + kTile * D;         // [G][D]
-  float* ps = qs + kMaxG * D;         // [G][kTile]
-  float* ms = ps + kMaxG * kTile;     // [G] running maximum, sum, factor
-  float* ls = ms + kMaxG;
-  float* fs = ls + kMaxG;
-  const int bh = blockIdx.x, tid = threadIdx.x, G = p.G;
-  const int cap = p.c.width * p.c.page;
-  int len = max(p.seqlens[bh], 0);
-  if (len > cap) {
-    if (tid == 0) set_error(p.c.err, WGKV_ERR_HEAD_CAPACITY);
-    len = cap;
+WGKV_DEV void mma_f16_16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+WGKV_DEV uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+WGKV_DEV uint32_t movmatrix_trans(uint32_t a) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+
+WGKV_DEV float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int D>
+__host__ __device__ constexpr int merge_row() { return D + 4; }  // D values, maximum, sum; rows 16 bytes apart mod 128
+
+size_t fixed_smem(int BH, int G, int D) {
+  return 128 + size_t(BH + 1 + kThreads) * 4 + size_t(kNCW) * G * (D + 4) * 4 + 2 * kMaxStages * 8 + 64;
+}
+
+// Tokens of head bh that count: not below 0, not past the table.
+WGKV_DEV int head_len(const Kv4DecodeParams& p, int bh) {
+  return min(max(__ldg(p.seqlens + bh), 0), p.c.width * p.c.page);
+}
+
+// kNT: 8-head tiles of query heads (G <= 8: 1, G <= 16: 2).
+template <int D, int NG, int kNT>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(Kv4DecodeParams p) {
+  using F = Kv4<D, NG>;
+  constexpr int W = D / 32;
+  constexpr int kMR = merge_row<D>();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* stage_base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+  const int S = p.stages, G = p.G, BH = p.BH;
+  float* merge = reinterpret_cast<float*>(stage_base + size_t(S) * kStageRecs * F::kRec);  // [kNCW][G][kMR]
+  uint64_t* full = reinterpret_cast<uint64_t*>(merge + kNCW * G * kMR);
+  uint64_t* empty = full + kMaxStages;
+  int* pre = reinterpret_cast<int*>(empty + kMaxStages);
+  int* scan = pre + BH + 1;
+  int* flag = scan + kThreads;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], kNCW);
+    }
+    fence_barrier_init();
   }
-  for (int e = tid; e < G * D; e += kThreads) qs[e] = bf2f(p.q[size_t(bh) * G * D + e]) * p.scale_log2;
-  if (tid < G) {
-    ms[tid] = -INFINITY;
-    ls[tid] = 0.f;
-  }
-  float acc[kMaxG];
-  for (int g = 0; g < kMaxG; ++g) acc[g] = 0.f;
-  for (int t0 = 0; t0 < len; t0 += kTile) {
-    const int n = min(kTile, len - t0);
+  griddep_wait();  // lengths, tables and rows may come from the launch just before
+  griddep_launch();
+
+  {  // first record of every head, in the line of all heads' records
+    const int per = (BH + kThreads - 1) / kThreads;
+    const int i0 = min(BH, tid * per), i1 = min(BH, i0 + per);
+    int sum = 0;
+    for (int i = i0; i < i1; ++i) {
+      sum += (head_len(p, i) + 15) >> 4;
+      if (blockIdx.x == 0 && __ldg(p.seqlens + i) > p.c.width * p.c.page) set_error(p.c.err, WGKV_ERR_HEAD_CAPACITY);
+    }
+    int total;
+    int run = block_excl_scan<kThreads>(sum, scan, total);
+    if (tid == 0) pre[BH] = total;
+    for (int i = i0; i < i1; ++i) {
+      pre[i] = run;
+      run += (head_len(p, i) + 15) >> 4;
+    }
     __syncthreads();
-    for (int e = tid; e < kTile * 4; e += kThreads) {
-      const int r = e >> 2, t = e & 3;
-      uint32_t kw[D / 32] = {}, vw[D / 32] = {}, kp[NG] = {}, vp[NG] = {};
-      if (r < n) {
-        const uint8_t* rec = kv4_record<D, NG>(p.c, bh, t0 + r);
-        if (rec) {
-          kv4_load_k<D, NG>(rec, (t0 + r) & 15, t, kw, kp);
-          kv4_load_v<D, NG>(rec, (t0 + r) & 15, t, vw, vp);
+  }
+  for (int bh = blockIdx.x; bh < BH; bh += gridDim.x) {  // heads that hold nothing
+    if (pre[bh + 1] == pre[bh])
+      for (int e = tid; e < G * D; e += kThreads) p.out[size_t(bh) * G * D + e] = 0;
+  }
+  const int U = pre[BH];
+  const int seg = (U + gridDim.x - 1) / gridDim.x;
+  const int u0 = min(U, int(blockIdx.x) * seg), u1 = min(U, u0 + seg);
+  if (u0 >= u1) return;
+  int lo = 0, hi = BH;  // pre[lo] <= u0 < pre[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (pre[mid] <= u0) lo = mid;
+    else hi = mid;
+  }
+
+  if (warp == 0) {
+    // ============================ producer ============================
+    // A step is up to kStageRecs consecutive records [b, b + n) of one head; lane i copies record i.
+    const int upp = p.c.page >> 4;
+    int bh = lo, b = u0;
+    auto fit = [&](int& n) {  // the step at (bh, b); false at the end of the segment
+      while (b < u1 && pre[bh + 1] <= b) ++bh;
+      n = b < u1 ? min(kStageRecs, min(u1, pre[bh + 1]) - b) : 0;
+      return n > 0;
+    };
+    auto place = [&](int n) -> int64_t {  // this lane's record in the cache, in records
+      if (lane >= n) return 0;
+      const int ul = b + lane - pre[bh];
+      int pid = __ldg(p.c.table + int64_t(bh) * p.c.table_stride + ul / upp);
+      if (pid < 0 || pid >= p.c.num_pages) {
+        set_error(p.c.err, WGKV_ERR_BAD_PAGE);
+        pid = 0;
+      }
+      return int64_t(pid) * upp + ul % upp;
+    };
+    int n, it = 0;
+    bool more = fit(n);
+    int64_t at = more ? place(n) : 0;
+    int s = 0;
+    uint32_t ph = 0;
+    while (more) {
+      const int n_now = n;
+      const int64_t at_now = at;
+      b += n;
+      more = fit(n);
+      if (more) at = place(n);  // in flight while this step waits for its stage
+      if (!mbar_wait(&empty[s], ph ^ 1)) {
+        set_error(p.c.err, WGKV_ERR_TIMEOUT);
+        break;
+      }
+      if (lane == 0) mbar_arrive_expect_tx(&full[s], n_now * F::kRec);
+      __syncwarp();
+      if (lane < n_now)
+        bulk_load(stage_base + (size_t(s) * kStageRecs + lane) * F::kRec, p.c.data + at_now * F::kRec, F::kRec,
+                  &full[s]);
+      __syncwarp();
+      ++it;
+      if (++s == S) s = 0, ph ^= 1;
+    }
+    // leave only once every copy this warp issued has landed (a consumer may have given up)
+    if (lane == 0) {
+      for (int j = max(0, it - S); j < it; ++j)
+        if (!mbar_wait(&full[j % S], (j / S) & 1)) set_error(p.c.err, WGKV_ERR_TIMEOUT);
+    }
+    return;
+  }
+
+  // ============================== consumers ==============================
+  const int cw = warp - 1, ctid = tid - 32;
+  const int g = lane >> 2, t4 = lane & 3;
+  int s = 0;
+  uint32_t ph = 0;
+  bool ok = true;
+  for (int bh = lo, rs = u0; rs < u1; ++bh) {
+    const int hs = pre[bh], he = pre[bh + 1];
+    if (he <= rs) continue;
+    const int re = min(u1, he);
+    const int len = head_len(p, bh);
+
+    // ---- queries: B fragments, power of two, sums over each group ----
+    uint32_t qf[kNT][W][4];       // [word of K][even k-step b0, b1, odd k-step b0, b1]
+    float qs[kNT][NG][2];         // scale_log2 * sum of the group's q, heads 2 t4 and 2 t4 + 1 of the tile
+    float alpha[kNT][2];          // what a product of codes and fragments is times x's scale
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+      const int head = nt * 8 + g;
+      float qv[W][8];
+      float big = 0.f;
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        uint4 raw = make_uint4(0, 0, 0, 0);
+        if (head < G) raw = __ldg(reinterpret_cast<const uint4*>(p.q + (size_t(bh) * G + head) * D + 32 * j + 8 * t4));
+        unpack8(raw, qv[j]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(qv[j][e]));
+      }
+      big = fmaxf(big, __shfl_xor_sync(0xffffffff, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffff, big, 2));
+      // 2^(14 - exponent(big)), it and its inverse times 2^24 kept normal numbers: smaller exponents count
+      // as -112; a query of 2^118 or more overflows (to NaN)
+      const int ex = min(max(int(__float_as_uint(big) >> 23) - 127, -112), 117);
+      const float up = __uint_as_float(uint32_t(14 - ex + 127) << 23);
+      float sum[NG];
+#pragma unroll
+      for (int n = 0; n < NG; ++n) sum[n] = 0.f;
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          sum[j * NG / W] += qv[j][e];
+          qv[j][e] *= up;
+        }
+        qf[nt][j][0] = pack_f16x2(qv[j][0], qv[j][4]);
+        qf[nt][j][1] = pack_f16x2(qv[j][2], qv[j][6]);
+        qf[nt][j][2] = pack_f16x2(qv[j][1] * 0.0625f, qv[j][5] * 0.0625f);
+        qf[nt][j][3] = pack_f16x2(qv[j][3] * 0.0625f, qv[j][7] * 0.0625f);
+      }
+      // 2^24 (the codes') / up (the queries'), as 2^(24 - 14 + ex): the lanes of heads 2 t4 and 2 t4 + 1 have it
+      const float a = p.scale_log2 * __uint_as_float(uint32_t(10 + ex + 127) << 23);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) alpha[nt][c] = __shfl_sync(0xffffffff, a, (2 * t4 + c) * 4);
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        sum[n] += __shfl_xor_sync(0xffffffff, sum[n], 1);
+        sum[n] += __shfl_xor_sync(0xffffffff, sum[n], 2);
+        sum[n] *= p.scale_log2;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) qs[nt][n][c] = __shfl_sync(0xffffffff, sum[n], (2 * t4 + c) * 4);
+      }
+    }
+
+    float acc[kNT][2 * W][4];     // O^T: m-tile, (dimension g: heads 2 t4, + 1; dimension g + 8: the same)
+    float um[kNT][NG][2];         // sum of p m_v over this lane's tokens
+    float mx[kNT][2], l[kNT][2];
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+      for (int m = 0; m < 2 * W; ++m) acc[nt][m][0] = acc[nt][m][1] = acc[nt][m][2] = acc[nt][m][3] = 0.f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        mx[nt][c] = -INFINITY;
+        l[nt][c] = 0.f;
+#pragma unroll
+        for (int n = 0; n < NG; ++n) um[nt][n][c] = 0.f;
+      }
+    }
+
+    for (int b0 = rs; b0 < re; b0 += kStageRecs) {
+      const int n = min(kStageRecs, re - b0);
+      const int per = (n + kNCW - 1) / kNCW;              // records of a warp in this step
+      const int r0 = min(n, cw * per), nb = min(per, n - r0);
+      if (ok && !mbar_wait(&full[s], ph)) {
+        set_error(p.c.err, WGKV_ERR_TIMEOUT);
+        ok = false;
+      }
+      if (ok && nb > 0) {
+        const uint8_t* recs = stage_base + (size_t(s) * kStageRecs + r0) * F::kRec;
+        const int left = len - (b0 + r0 - hs) * 16;       // tokens of the head from this warp's first record on
+        float x[kNB][kNT][4];
+        float top[kNT][2];
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
+        // ---- scores ----
+#pragma unroll
+        for (int i = 0; i < kNB; ++i) {
+          if (i < nb) {
+            const uint8_t* rec = recs + i * F::kRec;
+            uint32_t k0[W], k1[W], kp0[NG], kp1[NG];
+            ld_words<W>(k0, rec + lane * (D / 8));
+            ld_words<W>(k1, rec + 4 * D + lane * (D / 8));
+#pragma unroll
+            for (int n2 = 0; n2 < NG; ++n2) {
+              kp0[n2] = reinterpret_cast<const uint32_t*>(rec + F::kKP)[g * NG + n2];
+              kp1[n2] = reinterpret_cast<const uint32_t*>(rec + F::kKP)[(g + 8) * NG + n2];
+            }
+            float t[kNT][4], o[kNT][4];
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) t[nt][c] = o[nt][c] = 0.f;
+#pragma unroll
+            for (int n2 = 0; n2 < NG; ++n2) {
+              float d[kNT][4];
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt) d[nt][0] = d[nt][1] = d[nt][2] = d[nt][3] = 0.f;
+#pragma unroll
+              for (int j = n2 * (W / NG); j < (n2 + 1) * (W / NG); ++j) {
+                const uint32_t a = k0[j], b = k1[j], a8 = a >> 8, b8 = b >> 8;
+#pragma unroll
+                for (int nt = 0; nt < kNT; ++nt) {
+                  mma_f16_16816(d[nt], a & 0x000f000fu, b & 0x000f000fu, a8 & 0x000f000fu, b8 & 0x000f000fu,
+                                qf[nt][j][0], qf[nt][j][1]);
+                  mma_f16_16816(d[nt], a & 0x00f000f0u, b & 0x00f000f0u, a8 & 0x00f000f0u, b8 & 0x00f000f0u,
+                                qf[nt][j][2], qf[nt][j][3]);
+                }
+              }
+              const float s0 = __uint_as_float(kp0[n2] & 0xffff0000u), m0 = __uint_as_float(kp0[n2] << 16);
+              const float s1 = __uint_as_float(kp1[n2] & 0xffff0000u), m1 = __uint_as_float(kp1[n2] << 16);
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                  t[nt][c] = fmaf(s0, d[nt][c], t[nt][c]);
+                  t[nt][2 + c] = fmaf(s1, d[nt][2 + c], t[nt][2 + c]);
+                  o[nt][c] = fmaf(m0, qs[nt][n2][c], o[nt][c]);
+                  o[nt][2 + c] = fmaf(m1, qs[nt][n2][c], o[nt][2 + c]);
+                }
+              }
+            }
+            // exponent of the largest scale of the token's V row
+            uint32_t v0 = 0, v1 = 0;
+#pragma unroll
+            for (int n2 = 0; n2 < NG; ++n2) {
+              v0 = max(v0, reinterpret_cast<const uint32_t*>(rec + F::kVP)[g * NG + n2]);
+              v1 = max(v1, reinterpret_cast<const uint32_t*>(rec + F::kVP)[(g + 8) * NG + n2]);
+            }
+            const float e0 = fmaxf(__uint_as_float(0x4b000000u | v0 >> 23) - (8388608.f + 127.f), -40.f);
+            const float e1 = fmaxf(__uint_as_float(0x4b000000u | v1 >> 23) - (8388608.f + 127.f), -40.f);
+            const int valid = left - 16 * i;
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const float y = fmaf(alpha[nt][c & 1], t[nt][c], o[nt][c]);
+                x[i][nt][c] = g + 8 * (c >> 1) < valid ? y : -INFINITY;
+              }
+              top[nt][0] = fmaxf(top[nt][0], fmaxf(x[i][nt][0] + e0, x[i][nt][2] + e1));
+              top[nt][1] = fmaxf(top[nt][1], fmaxf(x[i][nt][1] + e0, x[i][nt][3] + e1));
+            }
+          }
+        }
+        // ---- reference ----
+        bool move = false;
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float m = top[nt][c];
+            m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 16));
+            top[nt][c] = m;
+            move |= m > mx[nt][c] + 8.f;
+          }
+        if (__any_sync(0xffffffff, move)) {
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float m = fmaxf(mx[nt][c], top[nt][c]);
+              const float f = mx[nt][c] == m ? 1.f : exp2_approx(mx[nt][c] - m);
+              mx[nt][c] = m;
+              l[nt][c] *= f;
+#pragma unroll
+              for (int n2 = 0; n2 < NG; ++n2) um[nt][n2][c] *= f;
+#pragma unroll
+              for (int m2 = 0; m2 < 2 * W; ++m2) {
+                acc[nt][m2][c] *= f;
+                acc[nt][m2][2 + c] *= f;
+              }
+            }
+        }
+        // ---- weights and O^T += C_v^T P^T ----
+#pragma unroll
+        for (int i = 0; i < kNB; ++i) {
+          if (i < nb) {
+            const uint8_t* rec = recs + i * F::kRec;
+            const int valid = left - 16 * i;
+            uint32_t v0[W], v1[W];
+            ld_words<W>(v0, rec + F::kV + lane * (D / 8));
+            ld_words<W>(v1, rec + F::kV + 4 * D + lane * (D / 8));
+            float pr[kNT][4];
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) pr[nt][c] = exp2_approx(x[i][nt][c] - mx[nt][c & 1]);
+              l[nt][0] += pr[nt][0] + pr[nt][2];
+              l[nt][1] += pr[nt][1] + pr[nt][3];
+            }
+#pragma unroll
+            for (int n2 = 0; n2 < NG; ++n2) {
+              uint32_t vp0 = reinterpret_cast<const uint32_t*>(rec + F::kVP)[g * NG + n2];
+              uint32_t vp1 = reinterpret_cast<const uint32_t*>(rec + F::kVP)[(g + 8) * NG + n2];
+              if (valid < 16) {  // places behind the length may hold anything
+                if (g >= valid) vp0 = 0;
+                if (g + 8 >= valid) vp1 = 0;
+              }
+              const float s0 = __uint_as_float(vp0 & 0xffff0000u), m0 = __uint_as_float(vp0 << 16);
+              const float s1 = __uint_as_float(vp1 & 0xffff0000u), m1 = __uint_as_float(vp1 << 16);
+              uint32_t pb[kNT][2];
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt) {
+                um[nt][n2][0] = fmaf(pr[nt][0], m0, fmaf(pr[nt][2], m1, um[nt][n2][0]));
+                um[nt][n2][1] = fmaf(pr[nt][1], m0, fmaf(pr[nt][3], m1, um[nt][n2][1]));
+                pb[nt][0] = movmatrix_trans(pack_f16x2(pr[nt][0] * s0, pr[nt][1] * s0));
+                pb[nt][1] = movmatrix_trans(pack_f16x2(pr[nt][2] * s1, pr[nt][3] * s1));
+              }
+#pragma unroll
+              for (int j = n2 * (W / NG); j < (n2 + 1) * (W / NG); ++j) {
+                const uint32_t a = v0[j], b = v1[j], a8 = a >> 8, b8 = b >> 8;
+#pragma unroll
+                for (int nt = 0; nt < kNT; ++nt) {
+                  mma_f16_16816(acc[nt][2 * j], a & 0x000f000fu, a8 & 0x000f000fu, b & 0x000f000fu, b8 & 0x000f000fu,
+                                pb[nt][0], pb[nt][1]);
+                  mma_f16_16816(acc[nt][2 * j + 1], a & 0x00f000f0u, a8 & 0x00f000f0u, b & 0x00f000f0u,
+                                b8 & 0x00f000f0u, pb[nt][0], pb[nt][1]);
+                }
+              }
+            }
+          }
         }
       }
-      for (int j = 0; j < D / 32; ++j)
-        for (int i = 0; i < 8; ++i) {
-          ks[r * (D + 1) + 32 * j + 8 * t + i] = kv4_value((kw[j] >> (4 * i)) & 15u, kp[j * NG / (D / 32)]);
-          vs[r * D + 32 * j + 8 * t + i] = kv4_value((vw[j] >> (4 * i)) & 15u, vp[j * NG / (D / 32)]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[s]);
+      if (++s == S) s = 0, ph ^= 1;
+    }
+
+    // ---- this warp's state of the head into shared memory ----
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int head = nt * 8 + 2 * t4 + c;
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          l[nt][c] += __shfl_xor_sync(0xffffffff, l[nt][c], o);
+#pragma unroll
+          for (int n2 = 0; n2 < NG; ++n2) um[nt][n2][c] += __shfl_xor_sync(0xffffffff, um[nt][n2][c], o);
         }
-    }
-    __syncthreads();
-    for (int e = tid; e < G * n; e += kThreads) {
-      const int g = e / n, r = e - g * n;
-      float s = 0.f;
-      for (int d = 0; d < D; ++d) s = fmaf(qs[g * D + d], ks[r * (D + 1) + d], s);
-      ps[g * kTile + r] = s;
-    }
-    __syncthreads();
-    if (tid < G) {
-      float m = ms[tid];
-      for (int r = 0; r < n; ++r) m = fmaxf(m, ps[tid * kTile + r]);
-      const float f = exp2f(ms[tid] - m);
-      float l = ls[tid] * f;
-      for (int r = 0; r < n; ++r) {
-        const float x = exp2f(ps[tid * kTile + r] - m);
-        ps[tid * kTile + r] = x;
-        l += x;
+        if (head < G) {
+          float* row = merge + (cw * G + head) * kMR;
+#pragma unroll
+          for (int j = 0; j < W; ++j) {
+            const float m = um[nt][j * NG / W][c];
+            float4 v;
+            v.x = fmaf(acc[nt][2 * j][c], 16777216.f, m);
+            v.y = fmaf(acc[nt][2 * j + 1][c], 1048576.f, m);
+            v.z = fmaf(acc[nt][2 * j][2 + c], 16777216.f, m);
+            v.w = fmaf(acc[nt][2 * j + 1][2 + c], 1048576.f, m);
+            *reinterpret_cast<float4*>(row + 32 * j + 4 * g) = v;
+          }
+          if (g == 0) {
+            row[D] = mx[nt][c];
+            row[D + 1] = l[nt][c];
+          }
+        }
       }
-      ms[tid] = m;
-      ls[tid] = l;
-      fs[tid] = f;
-    }
-    __syncthreads();
-    if (tid < D) {
-      for (int g = 0; g < G; ++g) {
-        float a = acc[g] * fs[g];
-        for (int r = 0; r < n; ++r) a = fmaf(ps[g * kTile + r], vs[r * D + tid], a);
-        acc[g] = a;
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kNCW));
+
+    const bool whole = rs == hs && re == he;
+    float* slot = p.part + size_t(bh + blockIdx.x) * G * (D + 2);
+    for (int e = ctid; e < G * D; e += 32 * kNCW) {
+      const int r = e / D, d = e - r * D;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kNCW; ++w) M = fmaxf(M, merge[(w * G + r) * kMR + D]);
+      float L = 0.f, A = 0.f;
+#pragma unroll
+      for (int w = 0; w < kNCW; ++w) {
+        const float* row = merge + (w * G + r) * kMR;
+        const float f = row[D] == M ? 1.f : exp2_approx(row[D] - M);
+        L = fmaf(row[D + 1], f, L);
+        A = fmaf(row[d], f, A);
+      }
+      if (whole) {
+        p.out[size_t(bh) * G * D + e] = f2bf(A / L);
+      } else {
+        slot[e] = A;
+        if (d == 0) {
+          slot[G * D + r] = M;
+          slot[G * D + G + r] = L;
+        }
       }
     }
+    if (!whole) {
+      __threadfence();
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * kNCW));
+      const int c_first = hs / seg, c_last = (he - 1) / seg;
+      if (ctid == 0) {
+        const int old = atomicAdd(&p.counters[bh], 1);
+        const int last = old == c_last - c_first;
+        if (last) p.counters[bh] = 0;
+        *flag = last;
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * kNCW));
+      if (*flag) {
+        __threadfence();
+        const float* p0 = p.part + size_t(bh + c_first) * G * (D + 2);
+        const int np = c_last - c_first + 1;
+        for (int e = ctid; e < G * D; e += 32 * kNCW) {
+          const int r = e / D;
+          float M = -INFINITY;
+          for (int c = 0; c < np; ++c) M = fmaxf(M, __ldcg(p0 + size_t(c) * G * (D + 2) + G * D + r));
+          float L = 0.f, A = 0.f;
+          for (int c = 0; c < np; ++c) {
+            const float* sl = p0 + size_t(c) * G * (D + 2);
+            const float mc = __ldcg(sl + G * D + r);
+            const float f = mc == M ? 1.f : exp2_approx(mc - M);
+            L = fmaf(__ldcg(sl + G * D + G + r), f, L);
+            A = fmaf(__ldcg(sl + e), f, A);
+          }
+          p.out[size_t(bh) * G * D + e] = f2bf(A / L);
+        }
+      }
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kNCW));  // merge rows free for the next head
+    rs = re;
   }
-  __syncthreads();
-  if (tid < D)
-    for (int g = 0; g < G; ++g)
-      p.out[(size_t(bh) * G + g) * D + tid] = f2bf(len > 0 ? acc[g] / ls[g] : 0.f);
+}
+
+size_t workspace_bytes(int64_t BH, int G, int D, int grid) {
+  return ((size_t(BH) * 4 + 255) & ~size_t(255)) + size_t(BH + grid) * G * (D + 2) * 4 + 256;
 }
 
 struct DecodeLaunch {
   Kv4DecodeParams p;
-  int BH;
+  void* ws;
   cudaStream_t stream;
-  int status;
-  template <int D, int NG>
-  void run() {
-    const size_t smem = (size_t(kTile) * (2 * D + 1) + kMaxG * D + kMaxG * kTile + 3 * kMaxG) * 4;
-    if (cudaFuncSetAttribute(kv4_decode_kernel<D, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) !=
-        cudaSuccess) {
-      status = WGKV_ECUDA;
+  int sms, status;
+  template <int D, int NG, int kNT>
+  void launch() {
+    const size_t stage = size_t(kStageRecs) * Kv4<D, NG>::kRec;
+    const size_t fixed = fixed_smem(p.BH, p.G, D);
+    // As many stages as fit next to another CTA; with many heads or a large group (their prefix sums and
+    // merge rows) a CTA has the SM to itself.
+    size_t room = ctas_per_sm(kNT) == 2 ? 227 * 1024 / 2 - 1024 : 227 * 1024;
+    if (fixed + 2 * stage > room) room = 227 * 1024;
+    if (fixed + 2 * stage > room) {
+      status = WGKV_EINVAL;
       return;
     }
-    kv4_decode_kernel<D, NG><<<BH, kThreads, smem, stream>>>(p);
-    status = cudaGetLastError() == cudaSuccess ? WGKV_OK : WGKV_ECUDA;
+    p.stages = int((room - fixed) / stage < size_t(kMaxStages) ? (room - fixed) / stage : size_t(kMaxStages));
+    static bool attr_set[64] = {false};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 64 || !attr_set[dev]) {
+      if (cudaFuncSetAttribute(kv4_decode_kernel<D, NG, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               227 * 1024) != cudaSuccess) {
+        status = WGKV_ECUDA;
+        return;
+      }
+      if (dev < 64) attr_set[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sms * ctas_per_sm(kNT));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = fixed + p.stages * stage;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // set-up overlaps the launch before
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    status = cudaLaunchKernelEx(&cfg, kv4_decode_kernel<D, NG, kNT>, p) == cudaSuccess ? WGKV_OK : WGKV_ECUDA;
+  }
+  template <int D, int NG>
+  void run() {
+    if (p.G <= 8) launch<D, NG, 1>();
+    else launch<D, NG, 2>();
   }
 };
+
 
 }  // namespace
 }  // namespace wgkv
@@ -125,7 +604,9 @@ struct DecodeLaunch {
 using namespace wgkv;
 
 extern "C" size_t wgkv_paged_decode_kv4_workspace_size(int batch, int num_q_heads, int num_kv_heads, int head_dim) {
-  return wgkv_paged_decode_workspace_size(batch, num_q_heads, num_kv_heads, head_dim);
+  if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || head_dim <= 0) return 0;
+  const int sms = device_sms(), G = num_q_heads / num_kv_heads;
+  return workspace_bytes(int64_t(batch) * num_kv_heads, G, head_dim, (sms > 0 ? sms : 148) * ctas_per_sm(G <= 8 ? 1 : 2));
 }
 
 extern "C" int wgkv_paged_decode_kv4(const uint16_t* q, const uint8_t* cache, int64_t num_pages, int page_size,
@@ -136,19 +617,30 @@ extern "C" int wgkv_paged_decode_kv4(const uint16_t* q, const uint8_t* cache, in
   if (!q || !cache || !cache_seqlens || !block_table || !out || !workspace || !kv4_supported(head_dim, group))
     return WGKV_EINVAL;
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads ||
-      num_q_heads / num_kv_heads > kMaxG || int64_t(batch) * num_kv_heads > 4096)
+      num_q_heads / num_kv_heads > kMaxG || int64_t(batch) * num_kv_heads > kMaxBH)
     return WGKV_EINVAL;
   if (num_pages <= 0 || page_size <= 0 || page_size % 16 || table_width <= 0 || table_stride < table_width ||
       int64_t(batch) * num_kv_heads * table_width * (page_size / 16) >= (int64_t(1) << 31) ||
       int64_t(table_width) * page_size >= (int64_t(1) << 31) ||
       (reinterpret_cast<uintptr_t>(cache) & 15) || (reinterpret_cast<uintptr_t>(q) & 15) ||
-      (reinterpret_cast<uintptr_t>(out) & 15))
+      (reinterpret_cast<uintptr_t>(out) & 15) || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return WGKV_EINVAL;
   if (workspace_bytes < wgkv_paged_decode_kv4_workspace_size(batch, num_q_heads, num_kv_heads, head_dim))
     return WGKV_ENOSPC;
-  DecodeLaunch a{{{const_cast<uint8_t*>(cache), num_pages, page_size, block_table, table_stride, table_width, err},
-                  q, out, cache_seqlens, num_q_heads / num_kv_heads, softmax_scale * 1.4426950408889634f},
-                 batch * num_kv_heads, as_stream(stream), WGKV_OK};
+  const int BH = batch * num_kv_heads;
+  DecodeLaunch a = {};
+  a.p.c = {const_cast<uint8_t*>(cache), num_pages, page_size, block_table, table_stride, table_width, err};
+  a.p.q = q;
+  a.p.out = out;
+  a.p.seqlens = cache_seqlens;
+  a.p.BH = BH;
+  a.p.G = num_q_heads / num_kv_heads;
+  a.p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  a.p.counters = reinterpret_cast<int*>(workspace);
+  a.p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ((size_t(BH) * 4 + 255) & ~size_t(255)));
+  a.stream = as_stream(stream);
+  a.sms = device_sms();
+  if (a.sms <= 0) return WGKV_ECUDA;
   kv4_dispatch(head_dim, group, a);
   return a.status;
 }
