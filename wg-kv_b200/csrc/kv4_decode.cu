@@ -49,7 +49,7 @@ struct Kv4DecodeParams {
   const int32_t* seqlens;
   int BH, G, stages;
   float scale_log2;
-  float* part;    // partial results: (BH + CTAs) x G x (D + 2)
+  float* part;    // partial results: (BH + CTAs) x G x (D + 4)
   int* counters;  // per head
 };
 
@@ -59,6 +59,16 @@ WGKV_DEV void mma_f16_16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uin
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same onto zero.
+WGKV_DEV void mma_f16_16816_first(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                  uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 WGKV_DEV uint32_t pack_f16x2(float lo, float hi) {
@@ -79,11 +89,43 @@ WGKV_DEV float exp2_approx(float x) {
   return y;
 }
 
+template <bool kB>
+struct Whole {
+  static constexpr bool value = kB;
+};
+
+template <int NG>
+WGKV_DEV void ld_pairs(uint32_t* w, const uint8_t* p) {
+  if (NG == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1 % NG] = v.y, w[2 % NG] = v.z, w[3 % NG] = v.w;
+  } else if (NG == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1 % NG] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
 template <int D>
 __host__ __device__ constexpr int merge_row() { return D + 4; }  // D values, maximum, sum; rows 16 bytes apart mod 128
 
-size_t fixed_smem(int BH, int G, int D) {
-  return 128 + size_t(BH + 1 + kThreads) * 4 + size_t(kNCW) * G * (D + 4) * 4 + 2 * kMaxStages * 8 + 64;
+WGKV_DEV void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kNCW) : "memory"); }
+
+// Four output values A / L; a head whose scores are all NaN has L = NaN.
+WGKV_DEV void store_out(uint16_t* out, const float4& A, float L) {
+  *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(A.x / L, A.y / L), pack_bf16x2(A.z / L, A.w / L));
+}
+
+// Floats that merging needs: a row per warp and query head, or two numbers per partial result and head.
+__host__ __device__ inline int merge_floats(int G, int D, int grid) {
+  const int a = kNCW * G * (D + 4), b = (2 * grid * G + 3) & ~3;
+  return a > b ? a : b;
+}
+
+size_t fixed_smem(int BH, int G, int D, int grid) {
+  return 128 + size_t(BH + 1 + kThreads) * 4 + size_t(merge_floats(G, D, grid)) * 4 + 32 * kNCW * 16 +
+         2 * kMaxStages * 8 + 64;
 }
 
 // Tokens of head bh that count: not below 0, not past the table.
@@ -101,7 +143,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
   uint8_t* stage_base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
   const int S = p.stages, G = p.G, BH = p.BH;
   float* merge = reinterpret_cast<float*>(stage_base + size_t(S) * kStageRecs * F::kRec);  // [kNCW][G][kMR]
-  uint64_t* full = reinterpret_cast<uint64_t*>(merge + kNCW * G * kMR);
+  float* join = merge + merge_floats(G, D, gridDim.x);                                                      // [32 kNCW][4]
+  uint64_t* full = reinterpret_cast<uint64_t*>(join + 32 * kNCW * 4);
   uint64_t* empty = full + kMaxStages;
   int* pre = reinterpret_cast<int*>(empty + kMaxStages);
   int* scan = pre + BH + 1;
@@ -140,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
       for (int e = tid; e < G * D; e += kThreads) p.out[size_t(bh) * G * D + e] = 0;
   }
   const int U = pre[BH];
-  const int seg = (U + gridDim.x - 1) / gridDim.x;
+  const int seg = max(kStageRecs, (U + int(gridDim.x) - 1) / int(gridDim.x));  // at least a stage
   const int u0 = min(U, int(blockIdx.x) * seg), u1 = min(U, u0 + seg);
   if (u0 >= u1) return;
   int lo = 0, hi = BH;  // pre[lo] <= u0 < pre[hi]
@@ -282,6 +325,160 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
       }
     }
 
+    // One step of this warp: nb records.  kAll: all kNB of them and every token counts, so that the records'
+    // instructions interleave.
+    auto step = [&](const uint8_t* recs, auto all, int nb, int left) {
+      constexpr bool kAll = decltype(all)::value;
+      float x[kNB][kNT][4];
+      float top[kNT][2];
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
+      // ---- scores ----
+#pragma unroll
+      for (int i = 0; i < kNB; ++i) {
+        if (!kAll && i >= nb) continue;
+        const uint8_t* rec = recs + i * F::kRec;
+        uint32_t k0[W], k1[W], kp0[NG], kp1[NG];
+        ld_words<W>(k0, rec + lane * (D / 8));
+        ld_words<W>(k1, rec + 4 * D + lane * (D / 8));
+        ld_pairs<NG>(kp0, rec + F::kKP + g * 4 * NG);
+        ld_pairs<NG>(kp1, rec + F::kKP + (g + 8) * 4 * NG);
+        float t[kNT][4], o[kNT][4];
+#pragma unroll
+        for (int n2 = 0; n2 < NG; ++n2) {
+          float d[kNT][4];
+#pragma unroll
+          for (int j = n2 * (W / NG); j < (n2 + 1) * (W / NG); ++j) {
+            const uint32_t a = k0[j], b = k1[j], a8 = a >> 8, b8 = b >> 8;
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt) {
+              if (j == n2 * (W / NG))
+                mma_f16_16816_first(d[nt], a & 0x000f000fu, b & 0x000f000fu, a8 & 0x000f000fu, b8 & 0x000f000fu,
+                                    qf[nt][j][0], qf[nt][j][1]);
+              else
+                mma_f16_16816(d[nt], a & 0x000f000fu, b & 0x000f000fu, a8 & 0x000f000fu, b8 & 0x000f000fu,
+                              qf[nt][j][0], qf[nt][j][1]);
+              mma_f16_16816(d[nt], a & 0x00f000f0u, b & 0x00f000f0u, a8 & 0x00f000f0u, b8 & 0x00f000f0u,
+                            qf[nt][j][2], qf[nt][j][3]);
+            }
+          }
+          const float s0 = __uint_as_float(kp0[n2] & 0xffff0000u), m0 = __uint_as_float(kp0[n2] << 16);
+          const float s1 = __uint_as_float(kp1[n2] & 0xffff0000u), m1 = __uint_as_float(kp1[n2] << 16);
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              t[nt][c] = n2 ? fmaf(s0, d[nt][c], t[nt][c]) : s0 * d[nt][c];
+              t[nt][2 + c] = n2 ? fmaf(s1, d[nt][2 + c], t[nt][2 + c]) : s1 * d[nt][2 + c];
+              o[nt][c] = n2 ? fmaf(m0, qs[nt][n2][c], o[nt][c]) : m0 * qs[nt][n2][c];
+              o[nt][2 + c] = n2 ? fmaf(m1, qs[nt][n2][c], o[nt][2 + c]) : m1 * qs[nt][n2][c];
+            }
+          }
+        }
+        // exponent of the largest scale of each token's V row
+        uint32_t vp0[NG], vp1[NG];
+        ld_pairs<NG>(vp0, rec + F::kVP + g * 4 * NG);
+        ld_pairs<NG>(vp1, rec + F::kVP + (g + 8) * 4 * NG);
+#pragma unroll
+        for (int n2 = 1; n2 < NG; ++n2) {
+          vp0[0] = max(vp0[0], vp0[n2]);
+          vp1[0] = max(vp1[0], vp1[n2]);
+        }
+        const float e0 = fmaxf(__uint_as_float(0x4b000000u | vp0[0] >> 23) - (8388608.f + 127.f), -40.f);
+        const float e1 = fmaxf(__uint_as_float(0x4b000000u | vp1[0] >> 23) - (8388608.f + 127.f), -40.f);
+        const int valid = left - 16 * i;
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float y = fmaf(alpha[nt][c & 1], t[nt][c], o[nt][c]);
+            x[i][nt][c] = kAll || g + 8 * (c >> 1) < valid ? y : -INFINITY;
+          }
+          top[nt][0] = fmaxf(top[nt][0], fmaxf(x[i][nt][0] + e0, x[i][nt][2] + e1));
+          top[nt][1] = fmaxf(top[nt][1], fmaxf(x[i][nt][1] + e0, x[i][nt][3] + e1));
+        }
+      }
+      // ---- reference ----
+      bool move = false;
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float m = top[nt][c];
+          m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 4));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 8));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 16));
+          top[nt][c] = m;
+          move |= m > mx[nt][c] + 8.f;
+        }
+      if (__any_sync(0xffffffff, move)) {
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float m = fmaxf(mx[nt][c], top[nt][c]);
+            const float f = mx[nt][c] == m ? 1.f : exp2_approx(mx[nt][c] - m);
+            mx[nt][c] = m;
+            l[nt][c] *= f;
+#pragma unroll
+            for (int n2 = 0; n2 < NG; ++n2) um[nt][n2][c] *= f;
+#pragma unroll
+            for (int m2 = 0; m2 < 2 * W; ++m2) {
+              acc[nt][m2][c] *= f;
+              acc[nt][m2][2 + c] *= f;
+            }
+          }
+      }
+      // ---- weights and O^T += C_v^T P^T ----
+#pragma unroll
+      for (int i = 0; i < kNB; ++i) {
+        if (!kAll && i >= nb) continue;
+        const uint8_t* rec = recs + i * F::kRec;
+        const int valid = left - 16 * i;
+        uint32_t v0[W], v1[W], vp0[NG], vp1[NG];
+        ld_words<W>(v0, rec + F::kV + lane * (D / 8));
+        ld_words<W>(v1, rec + F::kV + 4 * D + lane * (D / 8));
+        ld_pairs<NG>(vp0, rec + F::kVP + g * 4 * NG);
+        ld_pairs<NG>(vp1, rec + F::kVP + (g + 8) * 4 * NG);
+        float pr[kNT][4];
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) pr[nt][c] = exp2_approx(x[i][nt][c] - mx[nt][c & 1]);
+          l[nt][0] += pr[nt][0] + pr[nt][2];
+          l[nt][1] += pr[nt][1] + pr[nt][3];
+        }
+#pragma unroll
+        for (int n2 = 0; n2 < NG; ++n2) {
+          if (!kAll) {  // places behind the length may hold anything
+            if (g >= valid) vp0[n2] = 0;
+            if (g + 8 >= valid) vp1[n2] = 0;
+          }
+          const float s0 = __uint_as_float(vp0[n2] & 0xffff0000u), m0 = __uint_as_float(vp0[n2] << 16);
+          const float s1 = __uint_as_float(vp1[n2] & 0xffff0000u), m1 = __uint_as_float(vp1[n2] << 16);
+          uint32_t pb[kNT][2];
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt) {
+            um[nt][n2][0] = fmaf(pr[nt][0], m0, fmaf(pr[nt][2], m1, um[nt][n2][0]));
+            um[nt][n2][1] = fmaf(pr[nt][1], m0, fmaf(pr[nt][3], m1, um[nt][n2][1]));
+            pb[nt][0] = movmatrix_trans(pack_f16x2(pr[nt][0] * s0, pr[nt][1] * s0));
+            pb[nt][1] = movmatrix_trans(pack_f16x2(pr[nt][2] * s1, pr[nt][3] * s1));
+          }
+#pragma unroll
+          for (int j = n2 * (W / NG); j < (n2 + 1) * (W / NG); ++j) {
+            const uint32_t a = v0[j], b = v1[j], a8 = a >> 8, b8 = b >> 8;
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt) {
+              mma_f16_16816(acc[nt][2 * j], a & 0x000f000fu, a8 & 0x000f000fu, b & 0x000f000fu, b8 & 0x000f000fu,
+                            pb[nt][0], pb[nt][1]);
+              mma_f16_16816(acc[nt][2 * j + 1], a & 0x00f000f0u, a8 & 0x00f000f0u, b & 0x00f000f0u, b8 & 0x00f000f0u,
+                            pb[nt][0], pb[nt][1]);
+            }
+          }
+        }
+      }
+    };
+
     for (int b0 = rs; b0 < re; b0 += kStageRecs) {
       const int n = min(kStageRecs, re - b0);
       const int per = (n + kNCW - 1) / kNCW;              // records of a warp in this step
@@ -292,160 +489,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
       }
       if (ok && nb > 0) {
         const uint8_t* recs = stage_base + (size_t(s) * kStageRecs + r0) * F::kRec;
-        const int left = len - (b0 + r0 - hs) * 16;       // tokens of the head from this warp's first record on
-        float x[kNB][kNT][4];
-        float top[kNT][2];
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
-        // ---- scores ----
-#pragma unroll
-        for (int i = 0; i < kNB; ++i) {
-          if (i < nb) {
-            const uint8_t* rec = recs + i * F::kRec;
-            uint32_t k0[W], k1[W], kp0[NG], kp1[NG];
-            ld_words<W>(k0, rec + lane * (D / 8));
-            ld_words<W>(k1, rec + 4 * D + lane * (D / 8));
-#pragma unroll
-            for (int n2 = 0; n2 < NG; ++n2) {
-              kp0[n2] = reinterpret_cast<const uint32_t*>(rec + F::kKP)[g * NG + n2];
-              kp1[n2] = reinterpret_cast<const uint32_t*>(rec + F::kKP)[(g + 8) * NG + n2];
-            }
-            float t[kNT][4], o[kNT][4];
-#pragma unroll
-            for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) t[nt][c] = o[nt][c] = 0.f;
-#pragma unroll
-            for (int n2 = 0; n2 < NG; ++n2) {
-              float d[kNT][4];
-#pragma unroll
-              for (int nt = 0; nt < kNT; ++nt) d[nt][0] = d[nt][1] = d[nt][2] = d[nt][3] = 0.f;
-#pragma unroll
-              for (int j = n2 * (W / NG); j < (n2 + 1) * (W / NG); ++j) {
-                const uint32_t a = k0[j], b = k1[j], a8 = a >> 8, b8 = b >> 8;
-#pragma unroll
-                for (int nt = 0; nt < kNT; ++nt) {
-                  mma_f16_16816(d[nt], a & 0x000f000fu, b & 0x000f000fu, a8 & 0x000f000fu, b8 & 0x000f000fu,
-                                qf[nt][j][0], qf[nt][j][1]);
-                  mma_f16_16816(d[nt], a & 0x00f000f0u, b & 0x00f000f0u, a8 & 0x00f000f0u, b8 & 0x00f000f0u,
-                                qf[nt][j][2], qf[nt][j][3]);
-                }
-              }
-              const float s0 = __uint_as_float(kp0[n2] & 0xffff0000u), m0 = __uint_as_float(kp0[n2] << 16);
-              const float s1 = __uint_as_float(kp1[n2] & 0xffff0000u), m1 = __uint_as_float(kp1[n2] << 16);
-#pragma unroll
-              for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                  t[nt][c] = fmaf(s0, d[nt][c], t[nt][c]);
-                  t[nt][2 + c] = fmaf(s1, d[nt][2 + c], t[nt][2 + c]);
-                  o[nt][c] = fmaf(m0, qs[nt][n2][c], o[nt][c]);
-                  o[nt][2 + c] = fmaf(m1, qs[nt][n2][c], o[nt][2 + c]);
-                }
-              }
-            }
-            // exponent of the largest scale of the token's V row
-            uint32_t v0 = 0, v1 = 0;
-#pragma unroll
-            for (int n2 = 0; n2 < NG; ++n2) {
-              v0 = max(v0, reinterpret_cast<const uint32_t*>(rec + F::kVP)[g * NG + n2]);
-              v1 = max(v1, reinterpret_cast<const uint32_t*>(rec + F::kVP)[(g + 8) * NG + n2]);
-            }
-            const float e0 = fmaxf(__uint_as_float(0x4b000000u | v0 >> 23) - (8388608.f + 127.f), -40.f);
-            const float e1 = fmaxf(__uint_as_float(0x4b000000u | v1 >> 23) - (8388608.f + 127.f), -40.f);
-            const int valid = left - 16 * i;
-#pragma unroll
-            for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                const float y = fmaf(alpha[nt][c & 1], t[nt][c], o[nt][c]);
-                x[i][nt][c] = g + 8 * (c >> 1) < valid ? y : -INFINITY;
-              }
-              top[nt][0] = fmaxf(top[nt][0], fmaxf(x[i][nt][0] + e0, x[i][nt][2] + e1));
-              top[nt][1] = fmaxf(top[nt][1], fmaxf(x[i][nt][1] + e0, x[i][nt][3] + e1));
-            }
-          }
-        }
-        // ---- reference ----
-        bool move = false;
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float m = top[nt][c];
-            m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 4));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 8));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 16));
-            top[nt][c] = m;
-            move |= m > mx[nt][c] + 8.f;
-          }
-        if (__any_sync(0xffffffff, move)) {
-#pragma unroll
-          for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const float m = fmaxf(mx[nt][c], top[nt][c]);
-              const float f = mx[nt][c] == m ? 1.f : exp2_approx(mx[nt][c] - m);
-              mx[nt][c] = m;
-              l[nt][c] *= f;
-#pragma unroll
-              for (int n2 = 0; n2 < NG; ++n2) um[nt][n2][c] *= f;
-#pragma unroll
-              for (int m2 = 0; m2 < 2 * W; ++m2) {
-                acc[nt][m2][c] *= f;
-                acc[nt][m2][2 + c] *= f;
-              }
-            }
-        }
-        // ---- weights and O^T += C_v^T P^T ----
-#pragma unroll
-        for (int i = 0; i < kNB; ++i) {
-          if (i < nb) {
-            const uint8_t* rec = recs + i * F::kRec;
-            const int valid = left - 16 * i;
-            uint32_t v0[W], v1[W];
-            ld_words<W>(v0, rec + F::kV + lane * (D / 8));
-            ld_words<W>(v1, rec + F::kV + 4 * D + lane * (D / 8));
-            float pr[kNT][4];
-#pragma unroll
-            for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-              for (int c = 0; c < 4; ++c) pr[nt][c] = exp2_approx(x[i][nt][c] - mx[nt][c & 1]);
-              l[nt][0] += pr[nt][0] + pr[nt][2];
-              l[nt][1] += pr[nt][1] + pr[nt][3];
-            }
-#pragma unroll
-            for (int n2 = 0; n2 < NG; ++n2) {
-              uint32_t vp0 = reinterpret_cast<const uint32_t*>(rec + F::kVP)[g * NG + n2];
-              uint32_t vp1 = reinterpret_cast<const uint32_t*>(rec + F::kVP)[(g + 8) * NG + n2];
-              if (valid < 16) {  // places behind the length may hold anything
-                if (g >= valid) vp0 = 0;
-                if (g + 8 >= valid) vp1 = 0;
-              }
-              const float s0 = __uint_as_float(vp0 & 0xffff0000u), m0 = __uint_as_float(vp0 << 16);
-              const float s1 = __uint_as_float(vp1 & 0xffff0000u), m1 = __uint_as_float(vp1 << 16);
-              uint32_t pb[kNT][2];
-#pragma unroll
-              for (int nt = 0; nt < kNT; ++nt) {
-                um[nt][n2][0] = fmaf(pr[nt][0], m0, fmaf(pr[nt][2], m1, um[nt][n2][0]));
-                um[nt][n2][1] = fmaf(pr[nt][1], m0, fmaf(pr[nt][3], m1, um[nt][n2][1]));
-                pb[nt][0] = movmatrix_trans(pack_f16x2(pr[nt][0] * s0, pr[nt][1] * s0));
-                pb[nt][1] = movmatrix_trans(pack_f16x2(pr[nt][2] * s1, pr[nt][3] * s1));
-              }
-#pragma unroll
-              for (int j = n2 * (W / NG); j < (n2 + 1) * (W / NG); ++j) {
-                const uint32_t a = v0[j], b = v1[j], a8 = a >> 8, b8 = b >> 8;
-#pragma unroll
-                for (int nt = 0; nt < kNT; ++nt) {
-                  mma_f16_16816(acc[nt][2 * j], a & 0x000f000fu, a8 & 0x000f000fu, b & 0x000f000fu, b8 & 0x000f000fu,
-                                pb[nt][0], pb[nt][1]);
-                  mma_f16_16816(acc[nt][2 * j + 1], a & 0x00f000f0u, a8 & 0x00f000f0u, b & 0x00f000f0u,
-                                b8 & 0x00f000f0u, pb[nt][0], pb[nt][1]);
-                }
-              }
-            }
-          }
-        }
+        const int left = len - (b0 + r0 - hs) * 16;  // tokens of the head from this warp's first record on
+        if (nb == kNB && left >= 16 * kNB) step(recs, Whole<true>(), kNB, left);
+        else step(recs, Whole<false>(), nb, left);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
@@ -482,71 +528,107 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
           }
         }
       }
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * kNCW));
+    consumers_sync();
 
+    // ---- the warps' states into one: output, or this CTA's partial result ----
     const bool whole = rs == hs && re == he;
-    float* slot = p.part + size_t(bh + blockIdx.x) * G * (D + 2);
-    for (int e = ctid; e < G * D; e += 32 * kNCW) {
-      const int r = e / D, d = e - r * D;
+    float* slot = p.part + size_t(bh + blockIdx.x) * G * kMR;
+    for (int e = ctid; e < G * (D / 4); e += 32 * kNCW) {
+      const int r = e / (D / 4), d = 4 * (e % (D / 4));
+      const float* row = merge + r * kMR;
       float M = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kNCW; ++w) M = fmaxf(M, merge[(w * G + r) * kMR + D]);
-      float L = 0.f, A = 0.f;
+      for (int w = 0; w < kNCW; ++w) M = fmaxf(M, row[w * G * kMR + D]);
+      float L = 0.f;
+      float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kNCW; ++w) {
-        const float* row = merge + (w * G + r) * kMR;
-        const float f = row[D] == M ? 1.f : exp2_approx(row[D] - M);
-        L = fmaf(row[D + 1], f, L);
-        A = fmaf(row[d], f, A);
+        const float m = row[w * G * kMR + D];
+        const float f = m == M ? 1.f : exp2_approx(m - M);
+        const float4 v = *reinterpret_cast<const float4*>(row + w * G * kMR + d);
+        L = fmaf(row[w * G * kMR + D + 1], f, L);
+        A.x = fmaf(v.x, f, A.x), A.y = fmaf(v.y, f, A.y), A.z = fmaf(v.z, f, A.z), A.w = fmaf(v.w, f, A.w);
       }
       if (whole) {
-        p.out[size_t(bh) * G * D + e] = f2bf(A / L);
+        store_out(p.out + (size_t(bh) * G + r) * D + d, A, L);
       } else {
-        slot[e] = A;
-        if (d == 0) {
-          slot[G * D + r] = M;
-          slot[G * D + G + r] = L;
-        }
+        *reinterpret_cast<float4*>(slot + r * kMR + d) = A;
+        if (d == 0) *reinterpret_cast<float2*>(slot + r * kMR + D) = make_float2(M, L);
       }
     }
     if (!whole) {
       __threadfence();
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * kNCW));
-      const int c_first = hs / seg, c_last = (he - 1) / seg;
+      consumers_sync();
+      const int c_first = hs / seg, np = (he - 1) / seg - c_first + 1;
       if (ctid == 0) {
-        const int old = atomicAdd(&p.counters[bh], 1);
-        const int last = old == c_last - c_first;
+        const int last = atomicAdd(&p.counters[bh], 1) == np - 1;
         if (last) p.counters[bh] = 0;
         *flag = last;
       }
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * kNCW));
+      consumers_sync();
       if (*flag) {
         __threadfence();
-        const float* p0 = p.part + size_t(bh + c_first) * G * (D + 2);
-        const int np = c_last - c_first + 1;
-        for (int e = ctid; e < G * D; e += 32 * kNCW) {
-          const int r = e / D;
-          float M = -INFINITY;
-          for (int c = 0; c < np; ++c) M = fmaxf(M, __ldcg(p0 + size_t(c) * G * (D + 2) + G * D + r));
-          float L = 0.f, A = 0.f;
-          for (int c = 0; c < np; ++c) {
-            const float* sl = p0 + size_t(c) * G * (D + 2);
-            const float mc = __ldcg(sl + G * D + r);
-            const float f = mc == M ? 1.f : exp2_approx(mc - M);
-            L = fmaf(__ldcg(sl + G * D + G + r), f, L);
-            A = fmaf(__ldcg(sl + e), f, A);
+        const float* p0 = p.part + size_t(bh + c_first) * G * kMR;
+        float* fac = merge;            // [np][G]: each partial's maximum, then its factor
+        float* sum = fac + np * G;     // [np][G]
+        for (int e = ctid; e < np * G; e += 32 * kNCW) {
+          const float2 ml = __ldcg(reinterpret_cast<const float2*>(p0 + size_t(e) * kMR + D));
+          fac[e] = ml.x;
+          sum[e] = ml.y;
+        }
+        consumers_sync();
+        for (int r = cw; r < G; r += kNCW) {
+          float M = -INFINITY, L = 0.f;
+          for (int c = lane; c < np; c += 32) M = fmaxf(M, fac[c * G + r]);
+#pragma unroll
+          for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffff, M, o));
+          for (int c = lane; c < np; c += 32) {
+            const float m = fac[c * G + r], f = m == M ? 1.f : exp2_approx(m - M);
+            fac[c * G + r] = f;
+            L = fmaf(sum[c * G + r], f, L);
           }
-          p.out[size_t(bh) * G * D + e] = f2bf(A / L);
+#pragma unroll
+          for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffff, L, o);
+          __syncwarp();
+          if (lane == 0) sum[r] = L;  // only this warp reads row r of `sum`, and it is done
+        }
+        consumers_sync();
+        // a thread adds 4 dimensions over every `parts`-th partial
+        const int cols = G * (D / 4);
+        const int parts = 32 * kNCW / cols > 1 ? 32 * kNCW / cols : 1;
+        for (int e = ctid; e < cols * parts; e += 32 * kNCW) {
+          const int col = e % cols, part = e / cols, r = col / (D / 4), d = 4 * (col % (D / 4));
+          float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+          for (int c = part; c < np; c += parts) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(p0 + (size_t(c) * G + r) * kMR + d));
+            const float f = fac[c * G + r];
+            A.x = fmaf(v.x, f, A.x), A.y = fmaf(v.y, f, A.y), A.z = fmaf(v.z, f, A.z), A.w = fmaf(v.w, f, A.w);
+          }
+          if (parts == 1) store_out(p.out + (size_t(bh) * G + r) * D + d, A, sum[r]);
+          else reinterpret_cast<float4*>(join)[e] = A;
+        }
+        if (parts > 1) {
+          consumers_sync();
+          for (int e = ctid; e < cols; e += 32 * kNCW) {
+            const int r = e / (D / 4), d = 4 * (e % (D / 4));
+            float4 A = reinterpret_cast<const float4*>(join)[e];
+            for (int c = 1; c < parts; ++c) {
+              const float4 v = reinterpret_cast<const float4*>(join)[c * cols + e];
+              A.x += v.x, A.y += v.y, A.z += v.z, A.w += v.w;
+            }
+            store_out(p.out + (size_t(bh) * G + r) * D + d, A, sum[r]);
+          }
         }
       }
     }
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * kNCW));  // merge rows free for the next head
+    consumers_sync();  // merge rows free for the next head
     rs = re;
   }
 }
 
 size_t workspace_bytes(int64_t BH, int G, int D, int grid) {
-  return ((size_t(BH) * 4 + 255) & ~size_t(255)) + size_t(BH + grid) * G * (D + 2) * 4 + 256;
+  return ((size_t(BH) * 4 + 255) & ~size_t(255)) + size_t(BH + grid) * G * (D + 4) * 4 + 256;
 }
 
 struct DecodeLaunch {
@@ -557,7 +639,8 @@ struct DecodeLaunch {
   template <int D, int NG, int kNT>
   void launch() {
     const size_t stage = size_t(kStageRecs) * Kv4<D, NG>::kRec;
-    const size_t fixed = fixed_smem(p.BH, p.G, D);
+    const int grid = sms * ctas_per_sm(kNT);
+    const size_t fixed = fixed_smem(p.BH, p.G, D, grid);
     // As many stages as fit next to another CTA; with many heads or a large group (their prefix sums and
     // merge rows) a CTA has the SM to itself.
     size_t room = ctas_per_sm(kNT) == 2 ? 227 * 1024 / 2 - 1024 : 227 * 1024;
@@ -579,7 +662,7 @@ struct DecodeLaunch {
       if (dev < 64) attr_set[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(sms * ctas_per_sm(kNT));
+    cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = fixed + p.stages * stage;
     cfg.stream = stream;
