@@ -12,7 +12,8 @@
 // * A code is an fp16 operand without conversion: masked out of its word it is the subnormal code * 2^-24
 //   (bits 0-3) or code * 2^-20 (bits 4-7), which the tensor cores multiply exactly.  The factors are
 //   undone on q (odd k-steps carry q / 16) and on the output (odd m-tiles).  5 integer operations unpack
-//   8 codes.
+//   8 codes of K.  V takes 4: its even m-tiles get both codes of a byte, low + 16 high, and the odd ones'
+//   sums are subtracted at the end (in fp32, 17 times the low codes' rounding).
 // * q enters as fp16 times a power of two per head that puts its largest element in [2^14, 2^15): exact
 //   down to 2^-24 of it, 2^-36 of it absolute below.
 // * The weights p s_v are rounded to fp16 (11 bits).  The reference 2^r of p is a running maximum over
@@ -54,7 +55,7 @@ struct Kv4DecodeParams {
 };
 
 WGKV_DEV void mma_f16_16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -64,7 +65,7 @@ WGKV_DEV void mma_f16_16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uin
 // The same onto zero.
 WGKV_DEV void mma_f16_16816_first(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                   uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
@@ -79,13 +80,13 @@ WGKV_DEV uint32_t pack_f16x2(float lo, float hi) {
 
 WGKV_DEV uint32_t movmatrix_trans(uint32_t a) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
   return r;
 }
 
 WGKV_DEV float exp2_approx(float x) {
   float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -94,17 +95,16 @@ struct Whole {
   static constexpr bool value = kB;
 };
 
-template <int NG>
-WGKV_DEV void ld_pairs(uint32_t* w, const uint8_t* p) {
-  if (NG == 4) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    w[0] = v.x, w[1 % NG] = v.y, w[2 % NG] = v.z, w[3 % NG] = v.w;
-  } else if (NG == 2) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x, w[1 % NG] = v.y;
-  } else {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  }
+// N words from shared memory at byte address a (a multiple of 4 N).  The "memory" clobbers of the barrier
+// waits around them keep these loads in their stage.
+template <int N>
+WGKV_DEV void lds_words(uint32_t* w, uint32_t a) {
+  if (N == 4)
+    asm("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1 % N]), "=r"(w[2 % N]), "=r"(w[3 % N]) : "r"(a) : "memory");
+  else if (N == 2)
+    asm("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1 % N]) : "r"(a) : "memory");
+  else
+    asm("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(a) : "memory");
 }
 
 template <int D>
@@ -150,7 +150,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
   int* scan = pre + BH + 1;
   int* flag = scan + kThreads;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffff, tid >> 5, 0);  // the same in all lanes, so branches on it are uniform
+  const uint32_t stages = smem_u32(stage_base);
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
@@ -327,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
 
     // One step of this warp: nb records.  kAll: all kNB of them and every token counts, so that the records'
     // instructions interleave.
-    auto step = [&](const uint8_t* recs, auto all, int nb, int left) {
+    auto step = [&](uint32_t recs, auto all, int nb, int left) {
       constexpr bool kAll = decltype(all)::value;
       float x[kNB][kNT][4];
       float top[kNT][2];
@@ -337,12 +339,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
 #pragma unroll
       for (int i = 0; i < kNB; ++i) {
         if (!kAll && i >= nb) continue;
-        const uint8_t* rec = recs + i * F::kRec;
+        const uint32_t rec = recs + i * F::kRec;
         uint32_t k0[W], k1[W], kp0[NG], kp1[NG];
-        ld_words<W>(k0, rec + lane * (D / 8));
-        ld_words<W>(k1, rec + 4 * D + lane * (D / 8));
-        ld_pairs<NG>(kp0, rec + F::kKP + g * 4 * NG);
-        ld_pairs<NG>(kp1, rec + F::kKP + (g + 8) * 4 * NG);
+        lds_words<W>(k0, rec + lane * (D / 8));
+        lds_words<W>(k1, rec + 4 * D + lane * (D / 8));
+        lds_words<NG>(kp0, rec + F::kKP + g * 4 * NG);
+        lds_words<NG>(kp1, rec + F::kKP + (g + 8) * 4 * NG);
         float t[kNT][4], o[kNT][4];
 #pragma unroll
         for (int n2 = 0; n2 < NG; ++n2) {
@@ -377,8 +379,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
         }
         // exponent of the largest scale of each token's V row
         uint32_t vp0[NG], vp1[NG];
-        ld_pairs<NG>(vp0, rec + F::kVP + g * 4 * NG);
-        ld_pairs<NG>(vp1, rec + F::kVP + (g + 8) * 4 * NG);
+        lds_words<NG>(vp0, rec + F::kVP + g * 4 * NG);
+        lds_words<NG>(vp1, rec + F::kVP + (g + 8) * 4 * NG);
 #pragma unroll
         for (int n2 = 1; n2 < NG; ++n2) {
           vp0[0] = max(vp0[0], vp0[n2]);
@@ -433,13 +435,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
 #pragma unroll
       for (int i = 0; i < kNB; ++i) {
         if (!kAll && i >= nb) continue;
-        const uint8_t* rec = recs + i * F::kRec;
+        const uint32_t rec = recs + i * F::kRec;
         const int valid = left - 16 * i;
         uint32_t v0[W], v1[W], vp0[NG], vp1[NG];
-        ld_words<W>(v0, rec + F::kV + lane * (D / 8));
-        ld_words<W>(v1, rec + F::kV + 4 * D + lane * (D / 8));
-        ld_pairs<NG>(vp0, rec + F::kVP + g * 4 * NG);
-        ld_pairs<NG>(vp1, rec + F::kVP + (g + 8) * 4 * NG);
+        lds_words<W>(v0, rec + F::kV + lane * (D / 8));
+        lds_words<W>(v1, rec + F::kV + 4 * D + lane * (D / 8));
+        lds_words<NG>(vp0, rec + F::kVP + g * 4 * NG);
+        lds_words<NG>(vp1, rec + F::kVP + (g + 8) * 4 * NG);
         float pr[kNT][4];
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) {
@@ -466,11 +468,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
           }
 #pragma unroll
           for (int j = n2 * (W / NG); j < (n2 + 1) * (W / NG); ++j) {
-            const uint32_t a = v0[j], b = v1[j], a8 = a >> 8, b8 = b >> 8;
+            // two codes at a time: even rows of O^T get low + 16 high, odd rows 16 high
+            const uint32_t a = v0[j] & 0x00ff00ffu, b = v1[j] & 0x00ff00ffu;
+            const uint32_t a8 = __byte_perm(v0[j], 0, 0x4341), b8 = __byte_perm(v1[j], 0, 0x4341);
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt) {
-              mma_f16_16816(acc[nt][2 * j], a & 0x000f000fu, a8 & 0x000f000fu, b & 0x000f000fu, b8 & 0x000f000fu,
-                            pb[nt][0], pb[nt][1]);
+              mma_f16_16816(acc[nt][2 * j], a, a8, b, b8, pb[nt][0], pb[nt][1]);
               mma_f16_16816(acc[nt][2 * j + 1], a & 0x00f000f0u, a8 & 0x00f000f0u, b & 0x00f000f0u, b8 & 0x00f000f0u,
                             pb[nt][0], pb[nt][1]);
             }
@@ -488,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
         ok = false;
       }
       if (ok && nb > 0) {
-        const uint8_t* recs = stage_base + (size_t(s) * kStageRecs + r0) * F::kRec;
+        const uint32_t recs = stages + (s * kStageRecs + r0) * F::kRec;
         const int left = len - (b0 + r0 - hs) * 16;  // tokens of the head from this warp's first record on
         if (nb == kNB && left >= 16 * kNB) step(recs, Whole<true>(), kNB, left);
         else step(recs, Whole<false>(), nb, left);
@@ -516,9 +519,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
           for (int j = 0; j < W; ++j) {
             const float m = um[nt][j * NG / W][c];
             float4 v;
-            v.x = fmaf(acc[nt][2 * j][c], 16777216.f, m);
+            v.x = fmaf(acc[nt][2 * j][c] - acc[nt][2 * j + 1][c], 16777216.f, m);
             v.y = fmaf(acc[nt][2 * j + 1][c], 1048576.f, m);
-            v.z = fmaf(acc[nt][2 * j][2 + c], 16777216.f, m);
+            v.z = fmaf(acc[nt][2 * j][2 + c] - acc[nt][2 * j + 1][2 + c], 16777216.f, m);
             v.w = fmaf(acc[nt][2 * j + 1][2 + c], 1048576.f, m);
             *reinterpret_cast<float4*>(row + 32 * j + 4 * g) = v;
           }
