@@ -24,20 +24,22 @@
 //   packed weights, one per 8x8 block.
 //
 // Work is cut as in paged_decode.cu: the 16-token records of all heads laid end to end, equal segments per
-// CTA, one producer warp that copies whole records (cp.async.bulk, page ids loaded a step ahead) into a
-// ring of stages, consumer warps with up to kNB records each per stage; a head cut over CTAs is merged by
-// the last one to finish it (self-resetting counter, fixed order of summation).
+// CTA; a head cut over CTAs is merged by the last one to finish it (self-resetting counter, fixed order of
+// summation).  Inside a CTA every warp is on its own: it takes every kWarps-th pair of records of the
+// segment's part of a head, copies them itself (cp.async.bulk, one whole record each) into a ring of
+// slots of its own, a pair each, and works on a pair at a time; page ids are looked up 32 records at a
+// time, a batch ahead.  Warps meet only where a head ends.
 #include "kv4.cuh"
 #include "runtime.h"
 
 namespace wgkv {
 namespace {
 
-constexpr int kNCW = 7;                      // consumer warps; with the producer 8: 128 registers a thread at 2 CTAs per SM
-constexpr int kNB = 2;                       // records per consumer warp and stage
-constexpr int kStageRecs = kNCW * kNB;
-constexpr int kThreads = 32 * (kNCW + 1);
-constexpr int kMaxStages = 8;
+constexpr int kWarps = 8;                    // 128 registers a thread at 2 CTAs per SM
+constexpr int kNB = 2;                       // records of a slot, which a warp works on together
+constexpr int kThreads = 32 * kWarps;
+constexpr int kMaxSlots = 4;                 // slots of a warp's ring
+constexpr int kMinSegment = kWarps * kNB;    // records a CTA gets at least
 constexpr int kMaxBH = 4096;
 constexpr int kMaxG = 16;
 // CTAs per SM: the accumulators of two head tiles need the registers of the whole SM
@@ -48,7 +50,7 @@ struct Kv4DecodeParams {
   const uint16_t* q;
   uint16_t* out;
   const int32_t* seqlens;
-  int BH, G, stages;
+  int BH, G, slots;
   float scale_log2;
   float* part;    // partial results: (BH + CTAs) x G x (D + 4)
   int* counters;  // per head
@@ -110,8 +112,6 @@ WGKV_DEV void lds_words(uint32_t* w, uint32_t a) {
 template <int D>
 __host__ __device__ constexpr int merge_row() { return D + 4; }  // D values, maximum, sum; rows 16 bytes apart mod 128
 
-WGKV_DEV void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kNCW) : "memory"); }
-
 // Four output values A / L; a head whose scores are all NaN has L = NaN.
 WGKV_DEV void store_out(uint16_t* out, const float4& A, float L) {
   *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(A.x / L, A.y / L), pack_bf16x2(A.z / L, A.w / L));
@@ -119,13 +119,13 @@ WGKV_DEV void store_out(uint16_t* out, const float4& A, float L) {
 
 // Floats that merging needs: a row per warp and query head, or two numbers per partial result and head.
 __host__ __device__ inline int merge_floats(int G, int D, int grid) {
-  const int a = kNCW * G * (D + 4), b = (2 * grid * G + 3) & ~3;
+  const int a = kWarps * G * (D + 4), b = (2 * grid * G + 3) & ~3;
   return a > b ? a : b;
 }
 
 size_t fixed_smem(int BH, int G, int D, int grid) {
-  return 128 + size_t(BH + 1 + kThreads) * 4 + size_t(merge_floats(G, D, grid)) * 4 + 32 * kNCW * 16 +
-         2 * kMaxStages * 8 + 64;
+  return 128 + size_t(BH + 1 + kThreads) * 4 + size_t(merge_floats(G, D, grid)) * 4 + kThreads * 16 +
+         kWarps * kMaxSlots * 8 + 64;
 }
 
 // Tokens of head bh that count: not below 0, not past the table.
@@ -141,34 +141,30 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
   constexpr int kMR = merge_row<D>();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stage_base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
-  const int S = p.stages, G = p.G, BH = p.BH;
-  float* merge = reinterpret_cast<float*>(stage_base + size_t(S) * kStageRecs * F::kRec);  // [kNCW][G][kMR]
-  float* join = merge + merge_floats(G, D, gridDim.x);                                                      // [32 kNCW][4]
-  uint64_t* full = reinterpret_cast<uint64_t*>(join + 32 * kNCW * 4);
-  uint64_t* empty = full + kMaxStages;
-  int* pre = reinterpret_cast<int*>(empty + kMaxStages);
+  const int R = p.slots, G = p.G, BH = p.BH;
+  float* merge = reinterpret_cast<float*>(stage_base + size_t(kWarps) * R * kNB * F::kRec);  // [kWarps][G][kMR]
+  float* join = merge + merge_floats(G, D, gridDim.x);                                 // [kThreads][4]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(join + kThreads * 4);                   // [kWarps][kMaxSlots]
+  int* pre = reinterpret_cast<int*>(bars + kWarps * kMaxSlots);
   int* scan = pre + BH + 1;
   int* flag = scan + kThreads;
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffff, tid >> 5, 0);  // the same in all lanes, so branches on it are uniform
-  const uint32_t stages = smem_u32(stage_base);
-  if (tid == 0) {
-    for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], kNCW);
-    }
-    fence_barrier_init();
-  }
+  const uint32_t ring = smem_u32(stage_base) + warp * R * kNB * F::kRec;
+  uint64_t* full = bars + warp * kMaxSlots;
+  if (lane < R) mbar_init(&full[lane], 1);
+  fence_barrier_init();
   griddep_wait();  // lengths, tables and rows may come from the launch just before
   griddep_launch();
 
   {  // first record of every head, in the line of all heads' records
     const int per = (BH + kThreads - 1) / kThreads;
     const int i0 = min(BH, tid * per), i1 = min(BH, i0 + per);
-    int sum = 0;
+    int sum = 0, last = 0;
     for (int i = i0; i < i1; ++i) {
-      sum += (head_len(p, i) + 15) >> 4;
+      last = (head_len(p, i) + 15) >> 4;
+      sum += last;
       if (blockIdx.x == 0 && __ldg(p.seqlens + i) > p.c.width * p.c.page) set_error(p.c.err, WGKV_ERR_HEAD_CAPACITY);
     }
     int total;
@@ -176,7 +172,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
     if (tid == 0) pre[BH] = total;
     for (int i = i0; i < i1; ++i) {
       pre[i] = run;
-      run += (head_len(p, i) + 15) >> 4;
+      if (per > 1) last = (head_len(p, i) + 15) >> 4;
+      run += last;
     }
     __syncthreads();
   }
@@ -185,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
       for (int e = tid; e < G * D; e += kThreads) p.out[size_t(bh) * G * D + e] = 0;
   }
   const int U = pre[BH];
-  const int seg = max(kStageRecs, (U + int(gridDim.x) - 1) / int(gridDim.x));  // at least a stage
+  const int seg = max(kMinSegment, (U + int(gridDim.x) - 1) / int(gridDim.x));
   const int u0 = min(U, int(blockIdx.x) * seg), u1 = min(U, u0 + seg);
   if (u0 >= u1) return;
   int lo = 0, hi = BH;  // pre[lo] <= u0 < pre[hi]
@@ -195,62 +192,59 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
     else hi = mid;
   }
 
-  if (warp == 0) {
-    // ============================ producer ============================
-    // A step is up to kStageRecs consecutive records [b, b + n) of one head; lane i copies record i.
-    const int upp = p.c.page >> 4;
-    int bh = lo, b = u0;
-    auto fit = [&](int& n) {  // the step at (bh, b); false at the end of the segment
-      while (b < u1 && pre[bh + 1] <= b) ++bh;
-      n = b < u1 ? min(kStageRecs, min(u1, pre[bh + 1]) - b) : 0;
-      return n > 0;
-    };
-    auto place = [&](int n) -> int64_t {  // this lane's record in the cache, in records
-      if (lane >= n) return 0;
-      const int ul = b + lane - pre[bh];
-      int pid = __ldg(p.c.table + int64_t(bh) * p.c.table_stride + ul / upp);
-      if (pid < 0 || pid >= p.c.num_pages) {
-        set_error(p.c.err, WGKV_ERR_BAD_PAGE);
-        pid = 0;
-      }
-      return int64_t(pid) * upp + ul % upp;
-    };
-    int n, it = 0;
-    bool more = fit(n);
-    int64_t at = more ? place(n) : 0;
-    int s = 0;
-    uint32_t ph = 0;
-    while (more) {
-      const int n_now = n;
-      const int64_t at_now = at;
-      b += n;
-      more = fit(n);
-      if (more) at = place(n);  // in flight while this step waits for its stage
-      if (!mbar_wait(&empty[s], ph ^ 1)) {
-        set_error(p.c.err, WGKV_ERR_TIMEOUT);
+  // ---- this warp's records in order: of the pairs of each head's part of the segment, every kWarps-th ----
+  const int upp = p.c.page >> 4;
+  int f_bh = lo, f_off = 0;  // the next batch starts at this warp's pair f_off of head f_bh's part
+  auto fetch = [&]() -> int {  // 16 pairs, a record per lane: their places in the cache in records, -1 for none
+    int h = f_bh, o = f_off + (lane >> 1);
+    int at = -1;
+    while (h < BH && pre[h] < u1) {
+      const int first = max(pre[h], u0), pairs = (min(pre[h + 1], u1) - first + 1) >> 1;  // of all warps
+      const int c = (pairs - warp + kWarps - 1) / kWarps;
+      if (o < c) {
+        const int u = first + 2 * (warp + kWarps * o) + (lane & 1);
+        if (u < min(pre[h + 1], u1)) {
+          const int ul = u - pre[h];
+          int pid = __ldg(p.c.table + int64_t(h) * p.c.table_stride + ul / upp);
+          if (pid < 0 || pid >= p.c.num_pages) {
+            set_error(p.c.err, WGKV_ERR_BAD_PAGE);
+            pid = 0;
+          }
+          at = pid * upp + ul % upp;
+        }
         break;
       }
-      if (lane == 0) mbar_arrive_expect_tx(&full[s], n_now * F::kRec);
-      __syncwarp();
-      if (lane < n_now)
-        bulk_load(stage_base + (size_t(s) * kStageRecs + lane) * F::kRec, p.c.data + at_now * F::kRec, F::kRec,
-                  &full[s]);
-      __syncwarp();
-      ++it;
-      if (++s == S) s = 0, ph ^= 1;
+      o -= max(c, 0);
+      ++h;
     }
-    // leave only once every copy this warp issued has landed (a consumer may have given up)
-    if (lane == 0) {
-      for (int j = max(0, it - S); j < it; ++j)
-        if (!mbar_wait(&full[j % S], (j / S) & 1)) set_error(p.c.err, WGKV_ERR_TIMEOUT);
+    f_bh = __shfl_sync(0xffffffff, h, 31);
+    f_off = __shfl_sync(0xffffffff, o, 31) + 1;
+    return at;
+  };
+  int batch = fetch(), ahead = fetch(), used = 0;
+  int slot_in = 0, issued = 0, done = 0;
+  auto issue = [&]() {  // the next pair, if there is one, into slot slot_in
+    const int at = __shfl_sync(0xffffffff, batch, used + (lane & 1));
+    const uint32_t there = __ballot_sync(0xffffffff, at >= 0) & 3u;
+    if (there) {
+      if (lane == 0) mbar_arrive_expect_tx(&full[slot_in], there == 3u ? 2 * F::kRec : F::kRec);
+      if (lane < 2 && at >= 0)
+        bulk_load(stage_base + size_t((warp * R + slot_in) * kNB + lane) * F::kRec, p.c.data + int64_t(at) * F::kRec,
+                  F::kRec, &full[slot_in]);
+      ++issued;
     }
-    return;
-  }
+    slot_in = slot_in + 1 == R ? 0 : slot_in + 1;
+    used += 2;
+    if (used == 32) {
+      batch = ahead;
+      ahead = fetch();
+      used = 0;
+    }
+  };
+  for (int i = 0; i < R; ++i) issue();
 
-  // ============================== consumers ==============================
-  const int cw = warp - 1, ctid = tid - 32;
   const int g = lane >> 2, t4 = lane & 3;
-  int s = 0;
+  int slot = 0;       // the next pair's
   uint32_t ph = 0;
   bool ok = true;
   for (int bh = lo, rs = u0; rs < u1; ++bh) {
@@ -482,23 +476,25 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
       }
     };
 
-    for (int b0 = rs; b0 < re; b0 += kStageRecs) {
-      const int n = min(kStageRecs, re - b0);
-      const int per = (n + kNCW - 1) / kNCW;              // records of a warp in this step
-      const int r0 = min(n, cw * per), nb = min(per, n - r0);
-      if (ok && !mbar_wait(&full[s], ph)) {
-        set_error(p.c.err, WGKV_ERR_TIMEOUT);
+    const int pairs = (re - rs + 1) >> 1;
+    for (int i = warp; i < pairs; i += kWarps) {
+      if (!ok || !mbar_wait(&full[slot], ph)) {  // the head's result is lost; the counters below still come out right
+        if (ok) set_error(p.c.err, WGKV_ERR_TIMEOUT);
         ok = false;
+        break;
       }
-      if (ok && nb > 0) {
-        const uint32_t recs = stages + (s * kStageRecs + r0) * F::kRec;
-        const int left = len - (b0 + r0 - hs) * 16;  // tokens of the head from this warp's first record on
-        if (nb == kNB && left >= 16 * kNB) step(recs, Whole<true>(), kNB, left);
-        else step(recs, Whole<false>(), nb, left);
+      const uint32_t recs = ring + slot * (kNB * F::kRec);
+      slot = slot + 1 == R ? 0 : slot + 1;
+      ph ^= slot == 0;
+      ++done;
+      if (i + 1 < pairs) {
+        step(recs, Whole<true>(), kNB, 0);
+      } else {  // the part's last pair: one record, perhaps, and perhaps the head's end
+        const int u = rs + 2 * i;
+        step(recs, Whole<false>(), min(kNB, re - u), len - (u - hs) * 16);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[s]);
-      if (++s == S) s = 0, ph ^= 1;
+      __syncwarp();  // every lane has read the slot
+      issue();
     }
 
     // ---- this warp's state of the head into shared memory ----
@@ -514,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
           for (int n2 = 0; n2 < NG; ++n2) um[nt][n2][c] += __shfl_xor_sync(0xffffffff, um[nt][n2][c], o);
         }
         if (head < G) {
-          float* row = merge + (cw * G + head) * kMR;
+          float* row = merge + (warp * G + head) * kMR;
 #pragma unroll
           for (int j = 0; j < W; ++j) {
             const float m = um[nt][j * NG / W][c];
@@ -531,21 +527,21 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
           }
         }
       }
-    consumers_sync();
+    __syncthreads();
 
     // ---- the warps' states into one: output, or this CTA's partial result ----
     const bool whole = rs == hs && re == he;
     float* slot = p.part + size_t(bh + blockIdx.x) * G * kMR;
-    for (int e = ctid; e < G * (D / 4); e += 32 * kNCW) {
+    for (int e = tid; e < G * (D / 4); e += kThreads) {
       const int r = e / (D / 4), d = 4 * (e % (D / 4));
       const float* row = merge + r * kMR;
       float M = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kNCW; ++w) M = fmaxf(M, row[w * G * kMR + D]);
+      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, row[w * G * kMR + D]);
       float L = 0.f;
       float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kNCW; ++w) {
+      for (int w = 0; w < kWarps; ++w) {
         const float m = row[w * G * kMR + D];
         const float f = m == M ? 1.f : exp2_approx(m - M);
         const float4 v = *reinterpret_cast<const float4*>(row + w * G * kMR + d);
@@ -561,26 +557,26 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
     }
     if (!whole) {
       __threadfence();
-      consumers_sync();
+      __syncthreads();
       const int c_first = hs / seg, np = (he - 1) / seg - c_first + 1;
-      if (ctid == 0) {
+      if (tid == 0) {
         const int last = atomicAdd(&p.counters[bh], 1) == np - 1;
         if (last) p.counters[bh] = 0;
         *flag = last;
       }
-      consumers_sync();
+      __syncthreads();
       if (*flag) {
         __threadfence();
         const float* p0 = p.part + size_t(bh + c_first) * G * kMR;
         float* fac = merge;            // [np][G]: each partial's maximum, then its factor
         float* sum = fac + np * G;     // [np][G]
-        for (int e = ctid; e < np * G; e += 32 * kNCW) {
+        for (int e = tid; e < np * G; e += kThreads) {
           const float2 ml = __ldcg(reinterpret_cast<const float2*>(p0 + size_t(e) * kMR + D));
           fac[e] = ml.x;
           sum[e] = ml.y;
         }
-        consumers_sync();
-        for (int r = cw; r < G; r += kNCW) {
+        __syncthreads();
+        for (int r = warp; r < G; r += kWarps) {
           float M = -INFINITY, L = 0.f;
           for (int c = lane; c < np; c += 32) M = fmaxf(M, fac[c * G + r]);
 #pragma unroll
@@ -595,11 +591,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
           __syncwarp();
           if (lane == 0) sum[r] = L;  // only this warp reads row r of `sum`, and it is done
         }
-        consumers_sync();
+        __syncthreads();
         // a thread adds 4 dimensions over every `parts`-th partial
         const int cols = G * (D / 4);
-        const int parts = 32 * kNCW / cols > 1 ? 32 * kNCW / cols : 1;
-        for (int e = ctid; e < cols * parts; e += 32 * kNCW) {
+        const int parts = kThreads / cols > 1 ? kThreads / cols : 1;
+        for (int e = tid; e < cols * parts; e += kThreads) {
           const int col = e % cols, part = e / cols, r = col / (D / 4), d = 4 * (col % (D / 4));
           float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
@@ -612,8 +608,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
           else reinterpret_cast<float4*>(join)[e] = A;
         }
         if (parts > 1) {
-          consumers_sync();
-          for (int e = ctid; e < cols; e += 32 * kNCW) {
+          __syncthreads();
+          for (int e = tid; e < cols; e += kThreads) {
             const int r = e / (D / 4), d = 4 * (e % (D / 4));
             float4 A = reinterpret_cast<const float4*>(join)[e];
             for (int c = 1; c < parts; ++c) {
@@ -625,8 +621,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
         }
       }
     }
-    consumers_sync();  // merge rows free for the next head
+    __syncthreads();  // merge rows free for the next head
     rs = re;
+  }
+  // after a wait that gave up: leave only once every copy has landed
+  if (!ok && lane == 0) {
+    for (int i = done; i < issued; ++i) mbar_wait(&full[i % R], (i / R) & 1);
   }
 }
 
@@ -641,18 +641,18 @@ struct DecodeLaunch {
   int sms, status;
   template <int D, int NG, int kNT>
   void launch() {
-    const size_t stage = size_t(kStageRecs) * Kv4<D, NG>::kRec;
+    const size_t slot = size_t(kWarps) * kNB * Kv4<D, NG>::kRec;  // one more slot for every warp
     const int grid = sms * ctas_per_sm(kNT);
     const size_t fixed = fixed_smem(p.BH, p.G, D, grid);
-    // As many stages as fit next to another CTA; with many heads or a large group (their prefix sums and
+    // As many slots as fit next to another CTA; with many heads or a large group (their prefix sums and
     // merge rows) a CTA has the SM to itself.
     size_t room = ctas_per_sm(kNT) == 2 ? 227 * 1024 / 2 - 1024 : 227 * 1024;
-    if (fixed + 2 * stage > room) room = 227 * 1024;
-    if (fixed + 2 * stage > room) {
+    if (fixed + 2 * slot > room) room = 227 * 1024;
+    if (fixed + 2 * slot > room) {
       status = WGKV_EINVAL;
       return;
     }
-    p.stages = int((room - fixed) / stage < size_t(kMaxStages) ? (room - fixed) / stage : size_t(kMaxStages));
+    p.slots = int((room - fixed) / slot < size_t(kMaxSlots) ? (room - fixed) / slot : size_t(kMaxSlots));
     static bool attr_set[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -667,7 +667,7 @@ struct DecodeLaunch {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = fixed + p.stages * stage;
+    cfg.dynamicSmemBytes = fixed + p.slots * slot;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // set-up overlaps the launch before
@@ -707,7 +707,7 @@ extern "C" int wgkv_paged_decode_kv4(const uint16_t* q, const uint8_t* cache, in
     return WGKV_EINVAL;
   if (num_pages <= 0 || page_size <= 0 || page_size % 16 || table_width <= 0 || table_stride < table_width ||
       int64_t(batch) * num_kv_heads * table_width * (page_size / 16) >= (int64_t(1) << 31) ||
-      int64_t(table_width) * page_size >= (int64_t(1) << 31) ||
+      int64_t(table_width) * page_size >= (int64_t(1) << 31) || num_pages * (page_size / 16) >= (int64_t(1) << 31) ||
       (reinterpret_cast<uintptr_t>(cache) & 15) || (reinterpret_cast<uintptr_t>(q) & 15) ||
       (reinterpret_cast<uintptr_t>(out) & 15) || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return WGKV_EINVAL;
