@@ -35,7 +35,7 @@
 namespace wgkv {
 namespace {
 
-constexpr int kWarps = 8;                    // 128 registers a thread at 2 CTAs per SM
+constexpr int kWarps = 6;                    // 168 registers a thread at 2 CTAs per SM
 constexpr int kNB = 2;                       // records of a slot, which a warp works on together
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxSlots = 4;                 // slots of a warp's ring
@@ -222,7 +222,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
     return at;
   };
   int batch = fetch(), ahead = fetch(), used = 0;
-  int slot_in = 0, issued = 0, done = 0;
+  int slot_in = 0;
+  uint32_t flying = 0;  // slots whose copies nobody has waited for
   auto issue = [&]() {  // the next pair, if there is one, into slot slot_in
     const int at = __shfl_sync(0xffffffff, batch, used + (lane & 1));
     const uint32_t there = __ballot_sync(0xffffffff, at >= 0) & 3u;
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
       if (lane < 2 && at >= 0)
         bulk_load(stage_base + size_t((warp * R + slot_in) * kNB + lane) * F::kRec, p.c.data + int64_t(at) * F::kRec,
                   F::kRec, &full[slot_in]);
-      ++issued;
+      flying |= 1u << slot_in;
     }
     slot_in = slot_in + 1 == R ? 0 : slot_in + 1;
     used += 2;
@@ -251,7 +252,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
     const int hs = pre[bh], he = pre[bh + 1];
     if (he <= rs) continue;
     const int re = min(u1, he);
-    const int len = head_len(p, bh);
 
     // ---- queries: B fragments, power of two, sums over each group ----
     uint32_t qf[kNT][W][4];       // [word of K][even k-step b0, b1, odd k-step b0, b1]
@@ -314,22 +314,23 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
       for (int m = 0; m < 2 * W; ++m) acc[nt][m][0] = acc[nt][m][1] = acc[nt][m][2] = acc[nt][m][3] = 0.f;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        mx[nt][c] = -INFINITY;
+        mx[nt][c] = 0.f;
         l[nt][c] = 0.f;
 #pragma unroll
         for (int n = 0; n < NG; ++n) um[nt][n][c] = 0.f;
       }
     }
 
-    // One step of this warp: nb records.  kAll: all kNB of them and every token counts, so that the records'
-    // instructions interleave.
-    auto step = [&](uint32_t recs, auto all, int nb, int left) {
+    bool first = true;  // no reference yet
+    struct Scores {
+      float v[kNB][kNT][4];
+    };
+    // Scores of a pair of records relative to the reference, and a bound of their weights.  kAll: both are
+    // there and every token counts, so that nothing branches.
+    auto scores = [&](uint32_t recs, auto all, int nb, int left, Scores& x, float (&top)[kNT][2]) {
       constexpr bool kAll = decltype(all)::value;
-      float x[kNB][kNT][4];
-      float top[kNT][2];
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
-      // ---- scores ----
 #pragma unroll
       for (int i = 0; i < kNB; ++i) {
         if (!kAll && i >= nb) continue;
@@ -366,55 +367,60 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
             for (int c = 0; c < 2; ++c) {
               t[nt][c] = n2 ? fmaf(s0, d[nt][c], t[nt][c]) : s0 * d[nt][c];
               t[nt][2 + c] = n2 ? fmaf(s1, d[nt][2 + c], t[nt][2 + c]) : s1 * d[nt][2 + c];
-              o[nt][c] = n2 ? fmaf(m0, qs[nt][n2][c], o[nt][c]) : m0 * qs[nt][n2][c];
-              o[nt][2 + c] = n2 ? fmaf(m1, qs[nt][n2][c], o[nt][2 + c]) : m1 * qs[nt][n2][c];
+              o[nt][c] = fmaf(m0, qs[nt][n2][c], n2 ? o[nt][c] : -mx[nt][c]);
+              o[nt][2 + c] = fmaf(m1, qs[nt][n2][c], n2 ? o[nt][2 + c] : -mx[nt][c]);
             }
           }
         }
-        // exponent of the largest scale of each token's V row
+        // 2^23 + biased exponent of the largest scale of each token's V row (at least -40): added to x it
+        // rounds it to an integer, close enough for a bound
         uint32_t vp0[NG], vp1[NG];
         lds_words<NG>(vp0, rec + F::kVP + g * 4 * NG);
         lds_words<NG>(vp1, rec + F::kVP + (g + 8) * 4 * NG);
+        uint32_t v0 = uint32_t(127 - 40) << 23, v1 = v0;
 #pragma unroll
-        for (int n2 = 1; n2 < NG; ++n2) {
-          vp0[0] = max(vp0[0], vp0[n2]);
-          vp1[0] = max(vp1[0], vp1[n2]);
+        for (int n2 = 0; n2 < NG; ++n2) {
+          v0 = max(v0, vp0[n2]);
+          v1 = max(v1, vp1[n2]);
         }
-        const float e0 = fmaxf(__uint_as_float(0x4b000000u | vp0[0] >> 23) - (8388608.f + 127.f), -40.f);
-        const float e1 = fmaxf(__uint_as_float(0x4b000000u | vp1[0] >> 23) - (8388608.f + 127.f), -40.f);
+        const float e0 = __uint_as_float(0x4b000000u | v0 >> 23), e1 = __uint_as_float(0x4b000000u | v1 >> 23);
         const int valid = left - 16 * i;
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const float y = fmaf(alpha[nt][c & 1], t[nt][c], o[nt][c]);
-            x[i][nt][c] = kAll || g + 8 * (c >> 1) < valid ? y : -INFINITY;
+            x.v[i][nt][c] = kAll || g + 8 * (c >> 1) < valid ? y : -INFINITY;
           }
-          top[nt][0] = fmaxf(top[nt][0], fmaxf(x[i][nt][0] + e0, x[i][nt][2] + e1));
-          top[nt][1] = fmaxf(top[nt][1], fmaxf(x[i][nt][1] + e0, x[i][nt][3] + e1));
+          top[nt][0] = fmaxf(top[nt][0], fmaxf(x.v[i][nt][0] + e0, x.v[i][nt][2] + e1));
+          top[nt][1] = fmaxf(top[nt][1], fmaxf(x.v[i][nt][1] + e0, x.v[i][nt][3] + e1));
         }
       }
-      // ---- reference ----
-      bool move = false;
+    };
+    // Moves the reference where a weight would outgrow it: most pairs only learn that none does.
+    auto settle = [&](Scores& x, const float (&top)[kNT][2]) {
+      bool move = first;
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float m = top[nt][c];
-          m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 4));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 8));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 16));
-          top[nt][c] = m;
-          move |= m > mx[nt][c] + 8.f;
-        }
+      for (int nt = 0; nt < kNT; ++nt) move |= fmaxf(top[nt][0], top[nt][1]) > 8388608.f + 127.f + 8.f;
       if (__any_sync(0xffffffff, move)) {
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const float m = fmaxf(mx[nt][c], top[nt][c]);
-            const float f = mx[nt][c] == m ? 1.f : exp2_approx(mx[nt][c] - m);
-            mx[nt][c] = m;
+            float m = top[nt][c];
+            m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 16));
+            m -= 8388608.f + 127.f;
+            // up by `by`, where that is positive; the first time to where it belongs (a floor keeps it finite)
+            const float by = fmaxf(m, first ? -1e30f : 0.f);
+            const float f = first ? 0.f : exp2_approx(-by);
+            mx[nt][c] += by;
+#pragma unroll
+            for (int i = 0; i < kNB; ++i) {
+              x.v[i][nt][c] -= by;
+              x.v[i][nt][2 + c] -= by;
+            }
             l[nt][c] *= f;
 #pragma unroll
             for (int n2 = 0; n2 < NG; ++n2) um[nt][n2][c] *= f;
@@ -424,8 +430,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
               acc[nt][m2][2 + c] *= f;
             }
           }
+        first = false;
       }
-      // ---- weights and O^T += C_v^T P^T ----
+    };
+    // Weights, and O^T += C_v^T P^T.
+    auto weigh = [&](uint32_t recs, auto all, int nb, int left, const Scores& x) {
+      constexpr bool kAll = decltype(all)::value;
 #pragma unroll
       for (int i = 0; i < kNB; ++i) {
         if (!kAll && i >= nb) continue;
@@ -440,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) pr[nt][c] = exp2_approx(x[i][nt][c] - mx[nt][c & 1]);
+          for (int c = 0; c < 4; ++c) pr[nt][c] = exp2_approx(x.v[i][nt][c]);
           l[nt][0] += pr[nt][0] + pr[nt][2];
           l[nt][1] += pr[nt][1] + pr[nt][3];
         }
@@ -476,24 +486,53 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
       }
     };
 
+    // The scores of a pair are computed in one stretch of code with the weights and products of the one
+    // before, which do not depend on them; the part's last pair (one record, perhaps, and perhaps the head's
+    // end) goes by itself.
     const int pairs = (re - rs + 1) >> 1;
-    for (int i = warp; i < pairs; i += kWarps) {
-      if (!ok || !mbar_wait(&full[slot], ph)) {  // the head's result is lost; the counters below still come out right
-        if (ok) set_error(p.c.err, WGKV_ERR_TIMEOUT);
+    const int mine = (pairs - warp + kWarps - 1) / kWarps;                   // this warp's
+    const int whole_pairs = mine - (mine > 0 && (pairs - 1) % kWarps == warp);
+    auto arrived = [&](uint32_t& recs) -> bool {  // the next pair's slot, its copies landed
+      if (ok && !mbar_wait(&full[slot], ph)) {    // the head's result is lost; the counters below still come out right
+        set_error(p.c.err, WGKV_ERR_TIMEOUT);
         ok = false;
-        break;
       }
-      const uint32_t recs = ring + slot * (kNB * F::kRec);
+      if (!ok) return false;
+      recs = ring + slot * (kNB * F::kRec);
+      flying &= ~(1u << slot);
       slot = slot + 1 == R ? 0 : slot + 1;
       ph ^= slot == 0;
-      ++done;
-      if (i + 1 < pairs) {
-        step(recs, Whole<true>(), kNB, 0);
-      } else {  // the part's last pair: one record, perhaps, and perhaps the head's end
-        const int u = rs + 2 * i;
-        step(recs, Whole<false>(), min(kNB, re - u), len - (u - hs) * 16);
+      return true;
+    };
+    Scores x;
+    float top[kNT][2];
+    uint32_t now = 0, next = 0;
+    if (whole_pairs > 0 && arrived(now)) {
+      scores(now, Whole<true>(), kNB, 0, x, top);
+      settle(x, top);
+      for (int i = 1; i < whole_pairs && arrived(next); ++i) {
+        Scores y;
+        scores(next, Whole<true>(), kNB, 0, y, top);
+        weigh(now, Whole<true>(), kNB, 0, x);
+        __syncwarp();  // every lane has read the slot
+        issue();
+        settle(y, top);
+        x = y;
+        now = next;
       }
-      __syncwarp();  // every lane has read the slot
+      if (ok) {
+        weigh(now, Whole<true>(), kNB, 0, x);
+        __syncwarp();
+        issue();
+      }
+    }
+    if (mine > whole_pairs && arrived(now)) {
+      const int u = rs + 2 * (pairs - 1);
+      const int nb = min(kNB, re - u), left = head_len(p, bh) - (u - pre[bh]) * 16;
+      scores(now, Whole<false>(), nb, left, x, top);
+      settle(x, top);
+      weigh(now, Whole<false>(), nb, left, x);
+      __syncwarp();
       issue();
     }
 
@@ -522,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
             *reinterpret_cast<float4*>(row + 32 * j + 4 * g) = v;
           }
           if (g == 0) {
-            row[D] = mx[nt][c];
+            row[D] = first ? -INFINITY : mx[nt][c];
             row[D + 1] = l[nt][c];
           }
         }
@@ -626,7 +665,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
   }
   // after a wait that gave up: leave only once every copy has landed
   if (!ok && lane == 0) {
-    for (int i = done; i < issued; ++i) mbar_wait(&full[i % R], (i / R) & 1);
+    for (int i = 0; i < R; ++i)
+      if (flying >> i & 1u) mbar_wait(&full[i], i >= slot ? ph : ph ^ 1u);
   }
 }
 
