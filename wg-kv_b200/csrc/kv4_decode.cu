@@ -40,6 +40,7 @@ constexpr int kNB = 2;                       // records of a slot, which a warp 
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxSlots = 4;                 // slots of a warp's ring
 constexpr int kMinSegment = kWarps * kNB;    // records a CTA gets at least
+constexpr int kLaneHeads = 8;                // heads per lane up to which a warp sums up all lengths itself
 constexpr int kMaxBH = 4096;
 constexpr int kMaxG = 16;
 // CTAs per SM: the accumulators of two head tiles need the registers of the whole SM
@@ -112,20 +113,26 @@ WGKV_DEV void lds_words(uint32_t* w, uint32_t a) {
 template <int D>
 __host__ __device__ constexpr int merge_row() { return D + 4; }  // D values, maximum, sum; rows 16 bytes apart mod 128
 
+// What sums relative to reference m are worth relative to M >= m.
+WGKV_DEV float factor(float m, float M) { return m == M ? 1.f : exp2_approx(m - M); }
+
+// (A, L) += f (a, l), or = f (a, l).
+WGKV_DEV void add_state(float4& A, float& L, float f, const float4& a, float l, bool scale) {
+  L = scale ? f * l : fmaf(f, l, L);
+  A.x = scale ? f * a.x : fmaf(f, a.x, A.x);
+  A.y = scale ? f * a.y : fmaf(f, a.y, A.y);
+  A.z = scale ? f * a.z : fmaf(f, a.z, A.z);
+  A.w = scale ? f * a.w : fmaf(f, a.w, A.w);
+}
+
 // Four output values A / L; a head whose scores are all NaN has L = NaN.
 WGKV_DEV void store_out(uint16_t* out, const float4& A, float L) {
   *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(A.x / L, A.y / L), pack_bf16x2(A.z / L, A.w / L));
 }
 
-// Floats that merging needs: a row per warp and query head, or two numbers per partial result and head.
-__host__ __device__ inline int merge_floats(int G, int D, int grid) {
-  const int a = kWarps * G * (D + 4), b = (2 * grid * G + 3) & ~3;
-  return a > b ? a : b;
-}
-
-size_t fixed_smem(int BH, int G, int D, int grid) {
-  return 128 + size_t(BH + 1 + kThreads) * 4 + size_t(merge_floats(G, D, grid)) * 4 + kThreads * 16 +
-         kWarps * kMaxSlots * 8 + 64;
+size_t fixed_smem(int BH, int G, int D) {
+  return 128 + size_t(kWarps) * G * (D + 4) * 4 + kThreads * 32 + kWarps * kMaxSlots * 8 +
+         size_t(BH + 1 + kThreads) * 4 + 64;
 }
 
 // Tokens of head bh that count: not below 0, not past the table.
@@ -143,8 +150,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
   uint8_t* stage_base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
   const int R = p.slots, G = p.G, BH = p.BH;
   float* merge = reinterpret_cast<float*>(stage_base + size_t(kWarps) * R * kNB * F::kRec);  // [kWarps][G][kMR]
-  float* join = merge + merge_floats(G, D, gridDim.x);                                 // [kThreads][4]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(join + kThreads * 4);                   // [kWarps][kMaxSlots]
+  float* join = merge + kWarps * G * kMR;                                                   // [kThreads][8]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(join + kThreads * 8);                        // [kWarps][kMaxSlots]
   int* pre = reinterpret_cast<int*>(bars + kWarps * kMaxSlots);
   int* scan = pre + BH + 1;
   int* flag = scan + kThreads;
@@ -158,70 +165,111 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
   griddep_wait();  // lengths, tables and rows may come from the launch just before
   griddep_launch();
 
-  {  // first record of every head, in the line of all heads' records
+  // ---- pre[bh]: first record of head bh in the line of all heads' records ----
+  int U, lo;
+  int seg, u0, u1;
+  auto cut = [&]() {
+    seg = max(kMinSegment, (U + int(gridDim.x) - 1) / int(gridDim.x));
+    u0 = min(U, int(blockIdx.x) * seg);
+    u1 = min(U, u0 + seg);
+  };
+  if (BH <= 32 * kLaneHeads) {
+    // each warp for itself (all write the same values): no barrier between the launch and the first copy
+    const int per = (BH + 31) >> 5;
+    int n[kLaneHeads], sum = 0;
+#pragma unroll
+    for (int k = 0; k < kLaneHeads; ++k) {
+      const int i = lane * per + k;
+      n[k] = k < per && i < BH ? (head_len(p, i) + 15) >> 4 : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < kLaneHeads; ++k) sum += n[k];
+    int run = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffff, run, o);
+      if (lane >= o) run += y;
+    }
+    U = __shfl_sync(0xffffffff, run, 31);
+    run -= sum;
+    cut();
+    int before = 0;  // heads that begin at or before u0
+#pragma unroll
+    for (int k = 0; k < kLaneHeads; ++k) {
+      const int i = lane * per + k;
+      if (k < per && i < BH) {
+        pre[i] = run;
+        before += run <= u0;
+      }
+      run += n[k];
+    }
+    if (lane == 0) pre[BH] = U;
+    lo = __reduce_add_sync(0xffffffff, before) - 1;
+    __syncwarp();
+  } else {
     const int per = (BH + kThreads - 1) / kThreads;
     const int i0 = min(BH, tid * per), i1 = min(BH, i0 + per);
-    int sum = 0, last = 0;
-    for (int i = i0; i < i1; ++i) {
-      last = (head_len(p, i) + 15) >> 4;
-      sum += last;
-      if (blockIdx.x == 0 && __ldg(p.seqlens + i) > p.c.width * p.c.page) set_error(p.c.err, WGKV_ERR_HEAD_CAPACITY);
-    }
-    int total;
-    int run = block_excl_scan<kThreads>(sum, scan, total);
-    if (tid == 0) pre[BH] = total;
+    int sum = 0;
+    for (int i = i0; i < i1; ++i) sum += (head_len(p, i) + 15) >> 4;
+    int run = block_excl_scan<kThreads>(sum, scan, U);
+    if (tid == 0) pre[BH] = U;
     for (int i = i0; i < i1; ++i) {
       pre[i] = run;
-      if (per > 1) last = (head_len(p, i) + 15) >> 4;
-      run += last;
+      run += (head_len(p, i) + 15) >> 4;
     }
+    cut();
     __syncthreads();
+    int hi = BH;  // pre[lo] <= u0 < pre[hi]
+    lo = 0;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pre[mid] <= u0) lo = mid;
+      else hi = mid;
+    }
   }
-  for (int bh = blockIdx.x; bh < BH; bh += gridDim.x) {  // heads that hold nothing
+  for (int bh = blockIdx.x; bh < BH; bh += gridDim.x) {  // heads that hold nothing, lengths past the table
     if (pre[bh + 1] == pre[bh])
       for (int e = tid; e < G * D; e += kThreads) p.out[size_t(bh) * G * D + e] = 0;
+    if (tid == 0 && __ldg(p.seqlens + bh) > p.c.width * p.c.page) set_error(p.c.err, WGKV_ERR_HEAD_CAPACITY);
   }
-  const int U = pre[BH];
-  const int seg = max(kMinSegment, (U + int(gridDim.x) - 1) / int(gridDim.x));
-  const int u0 = min(U, int(blockIdx.x) * seg), u1 = min(U, u0 + seg);
   if (u0 >= u1) return;
-  int lo = 0, hi = BH;  // pre[lo] <= u0 < pre[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (pre[mid] <= u0) lo = mid;
-    else hi = mid;
-  }
 
   // ---- this warp's records in order: of the pairs of each head's part of the segment, every kWarps-th ----
   const int upp = p.c.page >> 4;
   int f_bh = lo, f_off = 0;  // the next batch starts at this warp's pair f_off of head f_bh's part
-  auto fetch = [&]() -> int {  // 16 pairs, a record per lane: their places in the cache in records, -1 for none
+  int f_page = 0, f_rec = -1;  // this lane's record of the batch fetched last: page id, as looked up, and place in it
+  auto fetch = [&]() {         // 16 pairs, a record per lane (f_rec -1 for none); nothing here waits for the lookup
     int h = f_bh, o = f_off + (lane >> 1);
-    int at = -1;
+    f_rec = -1;
     while (h < BH && pre[h] < u1) {
-      const int first = max(pre[h], u0), pairs = (min(pre[h + 1], u1) - first + 1) >> 1;  // of all warps
+      const int first = max(pre[h], u0), last = min(pre[h + 1], u1);
+      const int pairs = (last - first + 1) >> 1;  // of all warps
       const int c = (pairs - warp + kWarps - 1) / kWarps;
       if (o < c) {
         const int u = first + 2 * (warp + kWarps * o) + (lane & 1);
-        if (u < min(pre[h + 1], u1)) {
-          const int ul = u - pre[h];
-          int pid = __ldg(p.c.table + int64_t(h) * p.c.table_stride + ul / upp);
-          if (pid < 0 || pid >= p.c.num_pages) {
-            set_error(p.c.err, WGKV_ERR_BAD_PAGE);
-            pid = 0;
-          }
-          at = pid * upp + ul % upp;
+        if (u < last) {
+          const uint32_t ul = u - pre[h], pg = upp == 1 ? ul : ul / uint32_t(upp);
+          f_page = __ldg(p.c.table + int64_t(h) * p.c.table_stride + pg);
+          f_rec = ul - pg * upp;
         }
         break;
       }
-      o -= max(c, 0);
+      o -= c;
       ++h;
     }
     f_bh = __shfl_sync(0xffffffff, h, 31);
     f_off = __shfl_sync(0xffffffff, o, 31) + 1;
-    return at;
   };
-  int batch = fetch(), ahead = fetch(), used = 0;
+  auto resolve = [&]() -> int {  // its place in the cache, in records
+    if (f_rec < 0) return -1;
+    if (f_page < 0 || f_page >= p.c.num_pages) {
+      set_error(p.c.err, WGKV_ERR_BAD_PAGE);
+      f_page = 0;
+    }
+    return f_page * upp + f_rec;
+  };
+  fetch();
+  int batch = resolve(), used = 0;
   int slot_in = 0;
   uint32_t flying = 0;  // slots whose copies nobody has waited for
   auto issue = [&]() {  // the next pair, if there is one, into slot slot_in
@@ -237,12 +285,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
     slot_in = slot_in + 1 == R ? 0 : slot_in + 1;
     used += 2;
     if (used == 32) {
-      batch = ahead;
-      ahead = fetch();
+      batch = resolve();
+      fetch();
       used = 0;
     }
   };
   for (int i = 0; i < R; ++i) issue();
+  fetch();
 
   const int g = lane >> 2, t4 = lane & 3;
   int slot = 0;       // the next pair's
@@ -570,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
 
     // ---- the warps' states into one: output, or this CTA's partial result ----
     const bool whole = rs == hs && re == he;
-    float* slot = p.part + size_t(bh + blockIdx.x) * G * kMR;
+    float* mine_at = p.part + size_t(bh + blockIdx.x) * G * kMR;
     for (int e = tid; e < G * (D / 4); e += kThreads) {
       const int r = e / (D / 4), d = 4 * (e % (D / 4));
       const float* row = merge + r * kMR;
@@ -581,81 +630,75 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
       float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float m = row[w * G * kMR + D];
-        const float f = m == M ? 1.f : exp2_approx(m - M);
-        const float4 v = *reinterpret_cast<const float4*>(row + w * G * kMR + d);
-        L = fmaf(row[w * G * kMR + D + 1], f, L);
-        A.x = fmaf(v.x, f, A.x), A.y = fmaf(v.y, f, A.y), A.z = fmaf(v.z, f, A.z), A.w = fmaf(v.w, f, A.w);
+        const float* state = row + w * G * kMR;
+        add_state(A, L, factor(state[D], M), *reinterpret_cast<const float4*>(state + d), state[D + 1], false);
       }
       if (whole) {
         store_out(p.out + (size_t(bh) * G + r) * D + d, A, L);
       } else {
-        *reinterpret_cast<float4*>(slot + r * kMR + d) = A;
-        if (d == 0) *reinterpret_cast<float2*>(slot + r * kMR + D) = make_float2(M, L);
+        *reinterpret_cast<float4*>(mine_at + r * kMR + d) = A;
+        if (d == 0) *reinterpret_cast<float2*>(mine_at + r * kMR + D) = make_float2(M, L);
       }
     }
     if (!whole) {
-      __threadfence();
       __syncthreads();
       const int c_first = hs / seg, np = (he - 1) / seg - c_first + 1;
       if (tid == 0) {
+        __threadfence();  // the CTA's partial result, which the barrier put before this, ahead of the count
         const int last = atomicAdd(&p.counters[bh], 1) == np - 1;
         if (last) p.counters[bh] = 0;
+        __threadfence();
         *flag = last;
       }
       __syncthreads();
       if (*flag) {
-        __threadfence();
+        // a thread takes 4 dimensions of every `parts`-th partial result, kChunk loads in flight at once
+        constexpr int kChunk = 12;
         const float* p0 = p.part + size_t(bh + c_first) * G * kMR;
-        float* fac = merge;            // [np][G]: each partial's maximum, then its factor
-        float* sum = fac + np * G;     // [np][G]
-        for (int e = tid; e < np * G; e += kThreads) {
-          const float2 ml = __ldcg(reinterpret_cast<const float2*>(p0 + size_t(e) * kMR + D));
-          fac[e] = ml.x;
-          sum[e] = ml.y;
-        }
-        __syncthreads();
-        for (int r = warp; r < G; r += kWarps) {
-          float M = -INFINITY, L = 0.f;
-          for (int c = lane; c < np; c += 32) M = fmaxf(M, fac[c * G + r]);
-#pragma unroll
-          for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffff, M, o));
-          for (int c = lane; c < np; c += 32) {
-            const float m = fac[c * G + r], f = m == M ? 1.f : exp2_approx(m - M);
-            fac[c * G + r] = f;
-            L = fmaf(sum[c * G + r], f, L);
-          }
-#pragma unroll
-          for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffff, L, o);
-          __syncwarp();
-          if (lane == 0) sum[r] = L;  // only this warp reads row r of `sum`, and it is done
-        }
-        __syncthreads();
-        // a thread adds 4 dimensions over every `parts`-th partial
         const int cols = G * (D / 4);
         const int parts = kThreads / cols > 1 ? kThreads / cols : 1;
         for (int e = tid; e < cols * parts; e += kThreads) {
           const int col = e % cols, part = e / cols, r = col / (D / 4), d = 4 * (col % (D / 4));
+          float M = -INFINITY, L = 0.f;
           float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-          for (int c = part; c < np; c += parts) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p0 + (size_t(c) * G + r) * kMR + d));
-            const float f = fac[c * G + r];
-            A.x = fmaf(v.x, f, A.x), A.y = fmaf(v.y, f, A.y), A.z = fmaf(v.z, f, A.z), A.w = fmaf(v.w, f, A.w);
+          for (int c0 = part; c0 < np; c0 += kChunk * parts) {
+            float4 v[kChunk];
+            float2 ml[kChunk];
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) {
+              const int c = c0 + i * parts;
+              const float* row = p0 + (size_t(c) * G + r) * kMR;
+              ml[i] = c < np ? __ldcg(reinterpret_cast<const float2*>(row + D)) : make_float2(-INFINITY, 0.f);
+              v[i] = c < np ? __ldcg(reinterpret_cast<const float4*>(row + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            float m = M;
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) m = fmaxf(m, ml[i].x);
+            add_state(A, L, factor(M, m), A, L, true);
+            M = m;
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) add_state(A, L, factor(ml[i].x, m), v[i], ml[i].y, false);
           }
-          if (parts == 1) store_out(p.out + (size_t(bh) * G + r) * D + d, A, sum[r]);
-          else reinterpret_cast<float4*>(join)[e] = A;
+          if (parts == 1) {
+            store_out(p.out + (size_t(bh) * G + r) * D + d, A, L);
+          } else {
+            float* j = join + e * 8;
+            *reinterpret_cast<float4*>(j) = A;
+            *reinterpret_cast<float2*>(j + 4) = make_float2(M, L);
+          }
         }
         if (parts > 1) {
           __syncthreads();
           for (int e = tid; e < cols; e += kThreads) {
             const int r = e / (D / 4), d = 4 * (e % (D / 4));
-            float4 A = reinterpret_cast<const float4*>(join)[e];
-            for (int c = 1; c < parts; ++c) {
-              const float4 v = reinterpret_cast<const float4*>(join)[c * cols + e];
-              A.x += v.x, A.y += v.y, A.z += v.z, A.w += v.w;
+            float M = -INFINITY, L = 0.f;
+            float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int c = 0; c < parts; ++c) M = fmaxf(M, join[(c * cols + e) * 8 + 4]);
+            for (int c = 0; c < parts; ++c) {
+              const float* j = join + (c * cols + e) * 8;
+              add_state(A, L, factor(j[4], M), *reinterpret_cast<const float4*>(j), j[5], false);
             }
-            store_out(p.out + (size_t(bh) * G + r) * D + d, A, sum[r]);
+            store_out(p.out + (size_t(bh) * G + r) * D + d, A, L);
           }
         }
       }
@@ -683,7 +726,7 @@ struct DecodeLaunch {
   void launch() {
     const size_t slot = size_t(kWarps) * kNB * Kv4<D, NG>::kRec;  // one more slot for every warp
     const int grid = sms * ctas_per_sm(kNT);
-    const size_t fixed = fixed_smem(p.BH, p.G, D, grid);
+    const size_t fixed = fixed_smem(p.BH, p.G, D);
     // As many slots as fit next to another CTA; with many heads or a large group (their prefix sums and
     // merge rows) a CTA has the SM to itself.
     size_t room = ctas_per_sm(kNT) == 2 ? 227 * 1024 / 2 - 1024 : 227 * 1024;
