@@ -551,6 +551,22 @@ WGKV_API int wgkv_paged_decode_kv4(const uint16_t* q, const uint8_t* cache, int6
                                    int num_kv_heads, int head_dim, float softmax_scale, uint16_t* out,
                                    void* workspace, size_t workspace_bytes, int* err, void* stream);
 
+/*
+ * The three calls above with their arguments, in order, in an array of 8-byte slots (integers and pointers
+ * as int64, the softmax scale as a double): for bindings that convert arguments one by one and slowly (a
+ * ctypes call of 20 arguments costs more host time than the launch).  WGKV_EINVAL for another `op`.
+ */
+#define WGKV_KV4_APPEND 0       /* 23 slots */
+#define WGKV_KV4_READ 1         /* 17 slots */
+#define WGKV_KV4_PAGED_DECODE 2 /* 19 slots */
+WGKV_API int wgkv_kv4_call(int op, const void* slots);
+
+/*
+ * A number that tells the stream captures of a process apart (0: `stream` is not capturing).  Scratch that
+ * holds counters must be one graph's own: graphs captured on one stream may replay on several.
+ */
+WGKV_API uint64_t wgkv_stream_capture_id(void* stream);
+
 #ifdef __cplusplus
 }
 #endif

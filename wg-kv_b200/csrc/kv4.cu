@@ -1,4 +1,7 @@
 // Writing rows into the 4-bit KV cache and reading them back (format: kv4.cuh).
+#include <type_traits>
+#include <utility>
+
 #include "kv4.cuh"
 #include "runtime.h"
 
@@ -184,4 +187,52 @@ extern "C" int wgkv_kv4_read(const uint8_t* cache, int64_t num_pages, int page_s
                batch * kv_heads, rows, start, counts, out_k, out_v, as_stream(stream)};
   kv4_dispatch(head_dim, group, a);
   return cudaGetLastError() == cudaSuccess ? WGKV_OK : WGKV_ECUDA;
+}
+
+namespace {
+
+// Slot i of an argument array as a T.
+template <typename T>
+T slot(const void* slots, int i) {
+  const int64_t v = static_cast<const int64_t*>(slots)[i];
+  if constexpr (std::is_pointer<T>::value) return reinterpret_cast<T>(static_cast<intptr_t>(v));
+  else return static_cast<T>(v);
+}
+
+// the one floating argument travels as a double
+template <>
+float slot<float>(const void* slots, int i) {
+  return static_cast<float>(static_cast<const double*>(slots)[i]);
+}
+
+template <typename... Args, int... I>
+int call(int (*fn)(Args...), const void* slots, std::integer_sequence<int, I...>) {
+  return fn(slot<Args>(slots, I)...);
+}
+
+template <typename... Args>
+int call(int (*fn)(Args...), const void* slots) {
+  return call(fn, slots, std::make_integer_sequence<int, int(sizeof...(Args))>());
+}
+
+}  // namespace
+
+extern "C" int wgkv_kv4_call(int op, const void* slots) {
+  if (!slots) return WGKV_EINVAL;
+  switch (op) {
+    case WGKV_KV4_APPEND: return call(wgkv_kv4_append, slots);
+    case WGKV_KV4_READ: return call(wgkv_kv4_read, slots);
+    case WGKV_KV4_PAGED_DECODE: return call(wgkv_paged_decode_kv4, slots);
+    default: return WGKV_EINVAL;
+  }
+}
+
+extern "C" uint64_t wgkv_stream_capture_id(void* stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(as_stream(stream), &status, &id) != cudaSuccess) {
+    cudaGetLastError();  // the legacy stream beside another stream's capture: not captured itself
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusActive ? id : 0;
 }

@@ -19,10 +19,12 @@ through ``wgkv.check_errors()``.  The pool uses the same cache when ``init_pool`
 """
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from ._lib import check, lib
-from .runtime import err_word, require_cuda, stream_ptr, workspace
+from .runtime import counter_scratch, err_word, raw_stream, require_cuda
 
 GROUPS = {64: (32, 64), 128: (32, 64, 128)}  # head size -> group sizes
 _BY_ROW = {d + 8 * (d // g): (d, g) for d, gs in GROUPS.items() for g in gs}
@@ -43,71 +45,85 @@ def kv4_alloc(num_pages, page_size, head_dim, group_size=64, device="cuda"):
     return torch.zeros(num_pages, page_size, kv4_row_bytes(head_dim, group_size), dtype=torch.uint8, device=device)
 
 
+# wgkv_kv4_call's operations and the formats of their slots: the host's share of a small call is of the
+# order of the kernel, and converting 20 arguments one by one through ctypes is half of it
+_APPEND, _READ, _DECODE = 0, 1, 2
+_APPEND_SLOTS, _READ_SLOTS, _DECODE_SLOTS = struct.Struct("=23q"), struct.Struct("=17q"), struct.Struct("=13qd5q")
+_err_ptrs: dict = {}   # device index -> address of its error word
+_scratch: dict = {}    # (device index, B * Hk, G, D) -> (workspace bytes, bytes of counters) of paged_decode_kv4
+
+
 def _cache_dims(cache):
     """(head size, group size) of a cache tensor."""
+    if cache.dtype is torch.uint8 and cache.dim() == 3:
+        n, page, row = cache.shape
+        dims = _BY_ROW.get(row)
+        if dims is not None and n and page and page % 16 == 0:
+            if not cache.is_contiguous():
+                raise ValueError("a 4-bit cache must be contiguous")
+            return dims
     if cache.dtype != torch.uint8:
         raise TypeError(f"a 4-bit cache is a uint8 tensor, got {cache.dtype}")
-    if cache.dim() != 3 or cache.shape[2] not in _BY_ROW or cache.shape[0] == 0 or cache.shape[1] == 0 or \
-            cache.shape[1] % 16:
-        raise ValueError(f"a 4-bit cache is (num_pages, page_size, row_bytes) with page_size a multiple of 16 and "
-                         f"row_bytes one of {sorted(_BY_ROW)}, got {tuple(cache.shape)}")
-    if not cache.is_contiguous():
-        raise ValueError("a 4-bit cache must be contiguous")
-    return _BY_ROW[cache.shape[2]]
+    raise ValueError(f"a 4-bit cache is (num_pages, page_size, row_bytes) with page_size a multiple of 16 and "
+                     f"row_bytes one of {sorted(_BY_ROW)}, got {tuple(cache.shape)}")
 
 
-def _heads(t, name, B, Hk, dev):
-    """A (B, Hk) int32 tensor."""
-    if t.shape != (B, Hk):
-        raise ValueError(f"{name} must be (B, Hk) = ({B}, {Hk}), got {tuple(t.shape)}")
-    if t.device != dev:
-        raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
-    if t.dtype != torch.int32:
-        if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
+def _check_devices(cache, **tensors):
+    """All on the cache's GPU; returns its index."""
+    require_cuda(cache, "cache")
+    for name, t in tensors.items():
+        require_cuda(t, name)
+        if t.get_device() != cache.get_device():
+            raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
+    return cache.get_device()
+
+
+def _integers(t, name):
+    if t.dtype is not torch.int32:
+        if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype is torch.bool:
             raise TypeError(f"{name} must hold integers, got {t.dtype}")
         t = t.to(torch.int32)
+    return t
+
+
+def _heads(t, name, B, Hk):
+    """A (B, Hk) int32 tensor."""
+    if t.dim() != 2 or t.shape[0] != B or t.shape[1] != Hk:
+        raise ValueError(f"{name} must be (B, Hk) = ({B}, {Hk}), got {tuple(t.shape)}")
+    t = _integers(t, name)
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _table(t, dev):
-    """The block table (B, Hk, n) as int32 rows and their distance in elements."""
+def _table(t):
+    """The block table (B, Hk, n) as int32 rows, their distance in elements and its sizes."""
     if t.dim() != 3 or t.numel() == 0:
         raise ValueError(f"block_table must be (B, Hk, pages), none of them 0, got {tuple(t.shape)}")
-    if t.device != dev:
-        raise ValueError(f"block_table is on {t.device}, the cache on {dev}")
-    if t.dtype != torch.int32:
-        if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
-            raise TypeError(f"block_table must hold integers, got {t.dtype}")
-        t = t.to(torch.int32)
+    t = _integers(t, "block_table")
     B, Hk, w = t.shape
+    if t.is_contiguous():
+        return t, w, B, Hk, w
     rows = t.stride(1) if Hk > 1 else t.stride(0) if B > 1 else w
     if (w > 1 and t.stride(2) != 1) or rows < w or (B > 1 and Hk > 1 and t.stride(0) != Hk * rows):
         t, rows = t.contiguous(), w
-    return t, rows
+    return t, rows, B, Hk, w
 
 
-def _check_call(status, what, B, Hk, width, cache):
-    if status == -1:
-        if cache.data_ptr() % 16:
-            raise ValueError(f"{what}: the cache is not 16-byte aligned")
-        raise ValueError(f"{what}: refused sizes (B {B}, Hk {Hk}, table of {width} pages of {cache.shape[1]} tokens)")
-    check(status, what)
+def _call(index, op, slots, what, B, Hk, width, cache):
+    status = lib.wgkv_kv4_call(op, slots)
+    if status:
+        if status == -1:
+            if cache.data_ptr() % 16:
+                raise ValueError(f"{what}: the cache is not 16-byte aligned")
+            raise ValueError(f"{what}: refused sizes (B {B}, Hk {Hk}, table of {width} pages of {cache.shape[1]} "
+                             f"tokens, {cache.shape[0]} pages in the cache)")
+        check(status, what)
 
 
-class _on:
-    """The tensors' device as the current one (a no-op where it is already)."""
-    __slots__ = ("guard",)
-
-    def __init__(self, dev):
-        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _err_ptr(index):
+    p = _err_ptrs.get(index)
+    if p is None:
+        p = _err_ptrs[index] = err_word(torch.device("cuda", index)).data_ptr()
+    return p
 
 
 def kv4_append(k, v, cache, start, block_table, counts=None):
@@ -117,36 +133,37 @@ def kv4_append(k, v, cache, start, block_table, counts=None):
     counts (B, Hk) integers; rows ``r >= counts[b, h]`` are skipped (``counts=None``: none are).  Only the
     rows written change.  Rows past the head's table are dropped and reported by ``check_errors()``; no
     two rows of one call may name the same place.  Returns ``cache``."""
-    for t, n in ((k, "k"), (v, "v"), (cache, "cache"), (start, "start"), (block_table, "block_table")):
-        require_cuda(t, n)
+    index = _check_devices(cache, k=k, v=v, start=start, block_table=block_table)
     D, group = _cache_dims(cache)
-    dev = cache.device
-    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+    if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16:
         raise TypeError(f"k and v must be bf16, got {k.dtype} and {v.dtype}")
-    if k.dim() != 4 or k.shape != v.shape or k.shape[3] != D:
-        raise ValueError(f"k and v must be (B, Hk, L, {D}), got {tuple(k.shape)} and {tuple(v.shape)}")
-    if k.device != dev or v.device != dev:
-        raise ValueError(f"k is on {k.device}, v on {v.device}, the cache on {dev}")
-    B, Hk, L, _ = k.shape
-    if block_table.shape[:2] != (B, Hk):
-        raise ValueError(f"block_table must be ({B}, {Hk}, pages), got {tuple(block_table.shape)}")
-    start = _heads(start, "start", B, Hk, dev)
+    bt, bt_rows, B, Hk, width = _table(block_table)
+    if k.dim() != 4 or k.shape != v.shape or k.shape[3] != D or k.shape[0] != B or k.shape[1] != Hk:
+        raise ValueError(f"k and v must be ({B}, {Hk}, L, {D}), got {tuple(k.shape)} and {tuple(v.shape)}")
+    start = _heads(start, "start", B, Hk)
     if counts is not None:
-        require_cuda(counts, "counts")
-        counts = _heads(counts, "counts", B, Hk, dev)
-    bt, bt_rows = _table(block_table, dev)
+        _check_devices(cache, counts=counts)
+        counts = _heads(counts, "counts", B, Hk)
+    L = k.shape[2]
     if L == 0:
         return cache
-    if k.stride(3) != 1:
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return kv4_append(k, v, cache, start, block_table, counts)
+    k_sb, k_sh, k_st, k_sd = k.stride()
+    v_sb, v_sh, v_st, v_sd = v.stride()
+    if k_sd != 1:
         k = k.contiguous()
-    if v.stride(3) != 1:
+        k_sb, k_sh, k_st, _ = k.stride()
+    if v_sd != 1:
         v = v.contiguous()
-    with _on(dev):
-        st = lib.wgkv_kv4_append(k.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.data_ptr(), v.stride(0),
-                                 v.stride(1), v.stride(2), B, Hk, L, D, group, cache.data_ptr(), cache.shape[0],
-                                 cache.shape[1], start.data_ptr(), counts.data_ptr() if counts is not None else None,
-                                 bt.data_ptr(), bt_rows, bt.shape[2], err_word(dev).data_ptr(), stream_ptr(dev))
-    _check_call(st, "wgkv_kv4_append", B, Hk, bt.shape[2], cache)
+        v_sb, v_sh, v_st, _ = v.stride()
+    pages, page, _ = cache.shape
+    _call(index, _APPEND,
+          _APPEND_SLOTS.pack(k.data_ptr(), k_sb, k_sh, k_st, v.data_ptr(), v_sb, v_sh, v_st, B, Hk, L, D, group,
+                             cache.data_ptr(), pages, page, start.data_ptr(),
+                             counts.data_ptr() if counts is not None else 0, bt.data_ptr(), bt_rows, width,
+                             _err_ptr(index), raw_stream(index)), "wgkv_kv4_append", B, Hk, width, cache)
     return cache
 
 
@@ -156,56 +173,39 @@ def kv4_read(cache, start, counts, block_table, max_rows, out=None):
     Row i of (b, h) is logical position ``start[b, h] + i`` (``start=None``: i) for
     ``i < min(counts[b, h], max_rows)`` and zero behind that.  ``out``: two contiguous bf16 tensors to
     fill."""
-    for t, n in ((cache, "cache"), (counts, "counts"), (block_table, "block_table")):
-        require_cuda(t, n)
+    index = _check_devices(cache, counts=counts, block_table=block_table)
     D, group = _cache_dims(cache)
-    dev = cache.device
-    bt, bt_rows = _table(block_table, dev)
-    B, Hk, width = bt.shape
-    counts = _heads(counts, "counts", B, Hk, dev)
+    bt, bt_rows, B, Hk, width = _table(block_table)
+    counts = _heads(counts, "counts", B, Hk)
     if start is not None:
-        require_cuda(start, "start")
-        start = _heads(start, "start", B, Hk, dev)
+        _check_devices(cache, start=start)
+        start = _heads(start, "start", B, Hk)
     max_rows = int(max_rows)
     if max_rows < 0:
         raise ValueError(f"max_rows must not be negative, got {max_rows}")
     shape = (B, Hk, max_rows, D)
     if out is None:
-        ok, ov = (torch.empty(shape, dtype=torch.bfloat16, device=dev) for _ in range(2))
+        ok = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
+        ov = torch.empty_like(ok)
     else:
         ok, ov = out
         for t in (ok, ov):
-            if t.dtype != torch.bfloat16 or t.shape != shape or not t.is_contiguous() or t.device != dev:
-                raise ValueError(f"out must be two contiguous bf16 tensors {shape} on {dev}")
+            if t.dtype is not torch.bfloat16 or t.shape != shape or not t.is_contiguous() or t.device != cache.device:
+                raise ValueError(f"out must be two contiguous bf16 tensors {shape} on {cache.device}")
     if max_rows == 0:
         return ok, ov
-    if (ok.data_ptr() | ov.data_ptr()) % 16:
+    k_ptr, v_ptr = ok.data_ptr(), ov.data_ptr()
+    if (k_ptr | v_ptr) % 16:
         raise ValueError("out must be 16-byte aligned")
-    with _on(dev):
-        st = lib.wgkv_kv4_read(cache.data_ptr(), cache.shape[0], cache.shape[1], D, group,
-                               start.data_ptr() if start is not None else None, counts.data_ptr(), bt.data_ptr(),
-                               bt_rows, width, B, Hk, max_rows, ok.data_ptr(), ov.data_ptr(),
-                               err_word(dev).data_ptr(), stream_ptr(dev))
-    _check_call(st, "wgkv_kv4_read", B, Hk, width, cache)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return kv4_read(cache, start, counts, block_table, max_rows, (ok, ov))
+    pages, page, _ = cache.shape
+    _call(index, _READ,
+          _READ_SLOTS.pack(cache.data_ptr(), pages, page, D, group, start.data_ptr() if start is not None else 0,
+                           counts.data_ptr(), bt.data_ptr(), bt_rows, width, B, Hk, max_rows, k_ptr, v_ptr,
+                           _err_ptr(index), raw_stream(index)), "wgkv_kv4_read", B, Hk, width, cache)
     return ok, ov
-
-
-def _decode_args(q, cache, cache_seqlens, block_table):
-    D, group = _cache_dims(cache)
-    dev = cache.device
-    if q.dtype != torch.bfloat16:
-        raise TypeError(f"q must be bf16, got {q.dtype}")
-    if q.dim() != 4 or q.shape[1] != 1 or q.shape[3] != D:
-        raise ValueError(f"q must be (B, 1, Hq, {D}), got {tuple(q.shape)}")
-    if q.device != dev:
-        raise ValueError(f"q is on {q.device}, the cache on {dev}")
-    B, Hq = q.shape[0], q.shape[2]
-    if block_table.dim() != 3 or block_table.shape[0] != B:
-        raise ValueError(f"block_table must be (B, Hk, pages) with B = {B}, got {tuple(block_table.shape)}")
-    Hk = block_table.shape[1]
-    if Hk == 0 or Hq == 0 or Hq % Hk or Hq // Hk > 16:
-        raise ValueError(f"query heads ({Hq}) must be 1 to 16 times the KV heads ({Hk})")
-    return B, Hq, Hk, D, group, dev
 
 
 def paged_decode_kv4(q, cache, cache_seqlens, block_table, softmax_scale, out=None):
@@ -214,34 +214,42 @@ def paged_decode_kv4(q, cache, cache_seqlens, block_table, softmax_scale, out=No
 
     A head of length 0 gives zeros.  A length past the table's pages is cut there and reported by
     ``check_errors()``.  Hq / Hk at most 16; any B * Hk up to 4096."""
-    for t, n in ((q, "q"), (cache, "cache"), (cache_seqlens, "cache_seqlens"), (block_table, "block_table")):
-        require_cuda(t, n)
-    B, Hq, Hk, D, group, dev = _decode_args(q, cache, cache_seqlens, block_table)
-    sl = _heads(cache_seqlens, "cache_seqlens", B, Hk, dev)
-    bt, bt_rows = _table(block_table, dev)
+    index = _check_devices(cache, q=q, cache_seqlens=cache_seqlens, block_table=block_table)
+    D, group = _cache_dims(cache)
+    bt, bt_rows, B, Hk, width = _table(block_table)
+    if q.dtype is not torch.bfloat16:
+        raise TypeError(f"q must be bf16, got {q.dtype}")
+    if q.dim() != 4 or q.shape[0] != B or q.shape[1] != 1 or q.shape[3] != D:
+        raise ValueError(f"q must be ({B}, 1, Hq, {D}), got {tuple(q.shape)}")
+    Hq = q.shape[2]
+    if Hq == 0 or Hq % Hk or Hq > 16 * Hk:
+        raise ValueError(f"query heads ({Hq}) must be 1 to 16 times the KV heads ({Hk})")
+    sl = _heads(cache_seqlens, "cache_seqlens", B, Hk)
     if not q.is_contiguous():
         q = q.contiguous()
     if out is None:
         out = torch.empty_like(q)
-    elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous() or out.device != dev:
+    elif out.dtype is not torch.bfloat16 or out.shape != q.shape or not out.is_contiguous() or out.device != q.device:
         raise ValueError("out must be contiguous and like q")
     elif out.data_ptr() % 16:
         raise ValueError("out must be 16-byte aligned")
-    if q.data_ptr() % 16:
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return paged_decode_kv4(q, cache, cache_seqlens, block_table, softmax_scale, out)
+    q_ptr = q.data_ptr()
+    if q_ptr % 16:
         q = q.clone()
-    with _on(dev):
-        nbytes = int(lib.wgkv_paged_decode_kv4_workspace_size(B, Hq, Hk, D))
-        counters = ((B * Hk * 4 + 255) // 256) * 256
-        if torch.cuda.is_current_stream_capturing():
-            # a graph's own scratch (from its memory pool): graphs captured on one stream may replay on
-            # several, and must then not share the partial results and counters of the stream's scratch
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            ws[:counters].zero_()
-        else:
-            ws = workspace(dev, "paged_decode_kv4", nbytes, zero_prefix=counters)
-        st = lib.wgkv_paged_decode_kv4(q.data_ptr(), cache.data_ptr(), cache.shape[0], cache.shape[1], group,
-                                       sl.data_ptr(), bt.data_ptr(), bt_rows, bt.shape[2], B, Hq, Hk, D,
-                                       float(softmax_scale), out.data_ptr(), ws.data_ptr(), ws.numel(),
-                                       err_word(dev).data_ptr(), stream_ptr(dev))
-    _check_call(st, "wgkv_paged_decode_kv4", B, Hk, bt.shape[2], cache)
+        q_ptr = q.data_ptr()
+    key = (index, B * Hk, Hq // Hk, D)
+    need = _scratch.get(key)
+    if need is None:
+        need = _scratch[key] = (int(lib.wgkv_paged_decode_kv4_workspace_size(B, Hq, Hk, D)),
+                                (B * Hk * 4 + 255) // 256 * 256)
+    stream = raw_stream(index)
+    ws, ws_bytes = counter_scratch(index, stream, "paged_decode_kv4", *need)
+    pages, page, _ = cache.shape
+    _call(index, _DECODE,
+          _DECODE_SLOTS.pack(q_ptr, cache.data_ptr(), pages, page, group, sl.data_ptr(), bt.data_ptr(), bt_rows, width,
+                             B, Hq, Hk, D, softmax_scale, out.data_ptr(), ws, ws_bytes, _err_ptr(index), stream),
+          "wgkv_paged_decode_kv4", B, Hk, width, cache)
     return out

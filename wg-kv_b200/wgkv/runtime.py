@@ -22,6 +22,11 @@ def require_cuda(t: torch.Tensor, name: str):
         raise RuntimeError(f"{name} must be a CUDA tensor (this library has no CPU path)")
 
 
+def raw_stream(index: int) -> int:
+    """``stream_ptr`` of device ``index`` without building a Stream object (a C call)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def stream_ptr(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
@@ -67,6 +72,31 @@ def workspace(device, purpose: str, nbytes: int, zero_prefix: int = 0) -> torch.
     # this call's kernels may write anything past its own prefix and leave the prefix zero
     _workspaces[key] = (ws, zero_prefix)
     return ws
+
+
+_counter_scratch: dict = {}  # (device index, stream, purpose) -> [data pointer, bytes, zero prefix, tensor, capture id]
+
+
+def counter_scratch(index: int, stream: int, purpose: str, nbytes: int, zero_prefix: int):
+    """(pointer, bytes) of scratch of the current device whose first ``zero_prefix`` bytes are zero and are
+    left zero by the kernels that use it: :func:`workspace` for one raw stream, found with one dictionary
+    look-up, and safe under capture.  While a graph is captured its calls get scratch of the graph's own
+    (from its memory pool, zeroed by a node of the graph): graphs captured on one stream may replay on
+    several at a time, and must not share counters and partial results with one another or with the
+    stream's eager calls."""
+    capture = 0
+    key = (index, stream, purpose)
+    if torch.cuda.is_current_stream_capturing():
+        capture = lib.wgkv_stream_capture_id(stream)
+        key = (index, stream, purpose, "capture")
+    ent = _counter_scratch.get(key)
+    if ent is None or ent[1] < nbytes or ent[4] != capture:
+        t = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+        ent = _counter_scratch[key] = [t.data_ptr(), nbytes, 0, t, capture]
+    if ent[2] < zero_prefix:
+        ent[3][ent[2]:zero_prefix].zero_()  # stream-ordered, behind every earlier user on this stream
+    ent[2] = zero_prefix  # this call's kernels may write anything behind their own prefix
+    return ent[0], ent[1]
 
 
 def num_sms() -> int:
