@@ -35,16 +35,24 @@
 namespace wgkv {
 namespace {
 
-constexpr int kWarps = 6;                    // 168 registers a thread at 2 CTAs per SM
-constexpr int kNB = 2;                       // records of a slot, which a warp works on together
-constexpr int kThreads = 32 * kWarps;
-constexpr int kMaxSlots = 4;                 // slots of a warp's ring
-constexpr int kMinSegment = kWarps * kNB;    // records a CTA gets at least
-constexpr int kLaneHeads = 8;                // heads per lane up to which a warp sums up all lengths itself
+constexpr int kNB = 2;         // records of a slot, which a warp works on together
+constexpr int kMaxSlots = 4;   // slots of a warp's ring
+constexpr int kLaneHeads = 8;  // heads per lane up to which a warp sums up all lengths itself
 constexpr int kMaxBH = 4096;
 constexpr int kMaxG = 16;
-// CTAs per SM: the accumulators of two head tiles need the registers of the whole SM
-constexpr int ctas_per_sm(int head_tiles) { return head_tiles == 1 ? 2 : 1; }
+
+// Registers decide: 168 a thread for one tile of 8 query heads (2 CTAs of 6 warps per SM; 8 warps of 128
+// spill and are slower), 255 for two (one CTA of 8 warps).
+template <int kNT>
+struct Cfg {
+  static constexpr int kWarps = kNT == 1 ? 6 : 8;
+  static constexpr int kCtas = kNT == 1 ? 2 : 1;  // per SM
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kMinSegment = kWarps * kNB;  // records a CTA gets at least
+  // A CTA that meets a head's end spends about as long on the merge and the next head's start as on this
+  // many records: segments are cut at the heads' ends where that makes them no longer than this.
+  static constexpr int kAlignSlack = 16;
+};
 
 struct Kv4DecodeParams {
   Kv4Pages c;
@@ -116,13 +124,10 @@ __host__ __device__ constexpr int merge_row() { return D + 4; }  // D values, ma
 // What sums relative to reference m are worth relative to M >= m.
 WGKV_DEV float factor(float m, float M) { return m == M ? 1.f : exp2_approx(m - M); }
 
-// (A, L) += f (a, l), or = f (a, l).
-WGKV_DEV void add_state(float4& A, float& L, float f, const float4& a, float l, bool scale) {
-  L = scale ? f * l : fmaf(f, l, L);
-  A.x = scale ? f * a.x : fmaf(f, a.x, A.x);
-  A.y = scale ? f * a.y : fmaf(f, a.y, A.y);
-  A.z = scale ? f * a.z : fmaf(f, a.z, A.z);
-  A.w = scale ? f * a.w : fmaf(f, a.w, A.w);
+// (A, L) += f (a, l).
+WGKV_DEV void add_state(float4& A, float& L, float f, const float4& a, float l) {
+  L = fmaf(f, l, L);
+  A.x = fmaf(f, a.x, A.x), A.y = fmaf(f, a.y, A.y), A.z = fmaf(f, a.z, A.z), A.w = fmaf(f, a.w, A.w);
 }
 
 // Four output values A / L; a head whose scores are all NaN has L = NaN.
@@ -130,9 +135,9 @@ WGKV_DEV void store_out(uint16_t* out, const float4& A, float L) {
   *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(A.x / L, A.y / L), pack_bf16x2(A.z / L, A.w / L));
 }
 
-size_t fixed_smem(int BH, int G, int D) {
-  return 128 + size_t(kWarps) * G * (D + 4) * 4 + kThreads * 32 + kWarps * kMaxSlots * 8 +
-         size_t(BH + 1 + kThreads) * 4 + 64;
+size_t fixed_smem(int BH, int G, int D, int warps) {
+  return 128 + size_t(warps) * G * (D + 4) * 4 + warps * 32 * 32 + warps * kMaxSlots * 8 +
+         size_t(2 * BH + 32 * warps) * 4 + 64;
 }
 
 // Tokens of head bh that count: not below 0, not past the table.
@@ -142,8 +147,9 @@ WGKV_DEV int head_len(const Kv4DecodeParams& p, int bh) {
 
 // kNT: 8-head tiles of query heads (G <= 8: 1, G <= 16: 2).
 template <int D, int NG, int kNT>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(Kv4DecodeParams p) {
+__global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decode_kernel(Kv4DecodeParams p) {
   using F = Kv4<D, NG>;
+  constexpr int kWarps = Cfg<kNT>::kWarps, kThreads = Cfg<kNT>::kThreads;
   constexpr int W = D / 32;
   constexpr int kMR = merge_row<D>();
   extern __shared__ uint8_t smem_raw[];
@@ -152,8 +158,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
   float* merge = reinterpret_cast<float*>(stage_base + size_t(kWarps) * R * kNB * F::kRec);  // [kWarps][G][kMR]
   float* join = merge + kWarps * G * kMR;                                                   // [kThreads][8]
   uint64_t* bars = reinterpret_cast<uint64_t*>(join + kThreads * 8);                        // [kWarps][kMaxSlots]
-  int* pre = reinterpret_cast<int*>(bars + kWarps * kMaxSlots);
-  int* scan = pre + BH + 1;
+  int* pre = reinterpret_cast<int*>(bars + kWarps * kMaxSlots);  // [BH] a head's first record in the line
+  int* fin = pre + BH;                                           // [BH] the one behind its last
+  int* scan = fin + BH;
   int* flag = scan + kThreads;
 
   const int tid = threadIdx.x, lane = tid & 31;
@@ -165,61 +172,80 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
   griddep_wait();  // lengths, tables and rows may come from the launch just before
   griddep_launch();
 
-  // ---- pre[bh]: first record of head bh in the line of all heads' records ----
-  int U, lo;
-  int seg, u0, u1;
-  auto cut = [&]() {
-    seg = max(kMinSegment, (U + int(gridDim.x) - 1) / int(gridDim.x));
-    u0 = min(U, int(blockIdx.x) * seg);
-    u1 = min(U, u0 + seg);
-  };
+  // ---- the line of all heads' records and its cut into segments of `seg`, one per CTA ----
+  int seg, u0, u1, lo;
   if (BH <= 32 * kLaneHeads) {
     // each warp for itself (all write the same values): no barrier between the launch and the first copy
     const int per = (BH + 31) >> 5;
-    int n[kLaneHeads], sum = 0;
+    int n[kLaneHeads], room[kLaneHeads], sum = 0;
 #pragma unroll
     for (int k = 0; k < kLaneHeads; ++k) {
       const int i = lane * per + k;
       n[k] = k < per && i < BH ? (head_len(p, i) + 15) >> 4 : 0;
+      room[k] = n[k];
     }
 #pragma unroll
     for (int k = 0; k < kLaneHeads; ++k) sum += n[k];
+    const int U = __reduce_add_sync(0xffffffff, sum);
+    seg = max(Cfg<kNT>::kMinSegment, (U + int(gridDim.x) - 1) / int(gridDim.x));
+    // segments that end with the heads, if slightly longer ones are then few enough
+    if (U / (seg + Cfg<kNT>::kAlignSlack) + BH / 2 <= int(gridDim.x)) {
+      for (int more = 0; more <= Cfg<kNT>::kAlignSlack; more += more ? more : 2) {
+        const int longer = seg + more;
+        int ctas = 0;
+#pragma unroll
+        for (int k = 0; k < kLaneHeads; ++k)
+          if (k < per) ctas += (n[k] + longer - 1) / longer;
+        if (__reduce_add_sync(0xffffffff, ctas) > int(gridDim.x)) continue;
+        seg = longer;
+        sum = 0;
+#pragma unroll
+        for (int k = 0; k < kLaneHeads; ++k) {
+          if (k < per) room[k] = (n[k] + seg - 1) / seg * seg;
+          sum += room[k];
+        }
+        break;
+      }
+    }
     int run = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffff, run, o);
       if (lane >= o) run += y;
     }
-    U = __shfl_sync(0xffffffff, run, 31);
+    const int line = __shfl_sync(0xffffffff, run, 31);
     run -= sum;
-    cut();
+    u0 = min(line, int(blockIdx.x) * seg);
+    u1 = min(line, u0 + seg);
     int before = 0;  // heads that begin at or before u0
 #pragma unroll
     for (int k = 0; k < kLaneHeads; ++k) {
       const int i = lane * per + k;
       if (k < per && i < BH) {
         pre[i] = run;
+        fin[i] = run + n[k];
         before += run <= u0;
       }
-      run += n[k];
+      run += room[k];
     }
-    if (lane == 0) pre[BH] = U;
     lo = __reduce_add_sync(0xffffffff, before) - 1;
     __syncwarp();
   } else {
     const int per = (BH + kThreads - 1) / kThreads;
     const int i0 = min(BH, tid * per), i1 = min(BH, i0 + per);
-    int sum = 0;
+    int sum = 0, U;
     for (int i = i0; i < i1; ++i) sum += (head_len(p, i) + 15) >> 4;
     int run = block_excl_scan<kThreads>(sum, scan, U);
-    if (tid == 0) pre[BH] = U;
     for (int i = i0; i < i1; ++i) {
       pre[i] = run;
       run += (head_len(p, i) + 15) >> 4;
+      fin[i] = run;
     }
-    cut();
+    seg = max(Cfg<kNT>::kMinSegment, (U + int(gridDim.x) - 1) / int(gridDim.x));
+    u0 = min(U, int(blockIdx.x) * seg);
+    u1 = min(U, u0 + seg);
     __syncthreads();
-    int hi = BH;  // pre[lo] <= u0 < pre[hi]
+    int hi = BH;  // pre[lo] <= u0, and u0 < pre[hi] if there is a head hi
     lo = 0;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -228,11 +254,28 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
     }
   }
   for (int bh = blockIdx.x; bh < BH; bh += gridDim.x) {  // heads that hold nothing, lengths past the table
-    if (pre[bh + 1] == pre[bh])
+    if (fin[bh] == pre[bh])
       for (int e = tid; e < G * D; e += kThreads) p.out[size_t(bh) * G * D + e] = 0;
     if (tid == 0 && __ldg(p.seqlens + bh) > p.c.width * p.c.page) set_error(p.c.err, WGKV_ERR_HEAD_CAPACITY);
   }
   if (u0 >= u1) return;
+
+  // the queries of the first head are on their way while its pages are looked up
+  const int g = lane >> 2, t4 = lane & 3;
+  uint4 raw_q[kNT][W];
+  auto load_q = [&](int bh) {
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const int head = nt * 8 + g;
+        raw_q[nt][j] = make_uint4(0, 0, 0, 0);
+        if (head < G)
+          raw_q[nt][j] = __ldg(reinterpret_cast<const uint4*>(p.q + (size_t(bh) * G + head) * D + 32 * j + 8 * t4));
+      }
+  };
+  while (fin[lo] <= u0) ++lo;  // past heads that hold nothing
+  load_q(lo);
 
   // ---- this warp's records in order: of the pairs of each head's part of the segment, every kWarps-th ----
   const int upp = p.c.page >> 4;
@@ -242,8 +285,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
     int h = f_bh, o = f_off + (lane >> 1);
     f_rec = -1;
     while (h < BH && pre[h] < u1) {
-      const int first = max(pre[h], u0), last = min(pre[h + 1], u1);
-      const int pairs = (last - first + 1) >> 1;  // of all warps
+      const int first = max(pre[h], u0), last = min(fin[h], u1);
+      const int pairs = max(last - first + 1, 0) >> 1;  // of all warps
       const int c = (pairs - warp + kWarps - 1) / kWarps;
       if (o < c) {
         const int u = first + 2 * (warp + kWarps * o) + (lane & 1);
@@ -293,14 +336,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
   for (int i = 0; i < R; ++i) issue();
   fetch();
 
-  const int g = lane >> 2, t4 = lane & 3;
   int slot = 0;       // the next pair's
   uint32_t ph = 0;
   bool ok = true;
-  for (int bh = lo, rs = u0; rs < u1; ++bh) {
-    const int hs = pre[bh], he = pre[bh + 1];
-    if (he <= rs) continue;
-    const int re = min(u1, he);
+  for (int bh = lo; bh < BH && pre[bh] < u1; ++bh) {
+    const int hs = pre[bh], he = fin[bh];
+    const int rs = max(hs, u0), re = min(he, u1);
+    if (re <= rs) continue;
 
     // ---- queries: B fragments, power of two, sums over each group ----
     uint32_t qf[kNT][W][4];       // [word of K][even k-step b0, b1, odd k-step b0, b1]
@@ -308,14 +350,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
     float alpha[kNT][2];          // what a product of codes and fragments is times x's scale
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
-      const int head = nt * 8 + g;
       float qv[W][8];
       float big = 0.f;
 #pragma unroll
       for (int j = 0; j < W; ++j) {
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (head < G) raw = __ldg(reinterpret_cast<const uint4*>(p.q + (size_t(bh) * G + head) * D + 32 * j + 8 * t4));
-        unpack8(raw, qv[j]);
+        unpack8(raw_q[nt][j], qv[j]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(qv[j][e]));
       }
@@ -585,7 +624,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
       issue();
     }
 
-    // ---- this warp's state of the head into shared memory ----
+    // ---- this warp's state of the head into shared memory, the next head's queries on their way ----
+    int after = bh + 1;
+    while (after < BH && fin[after] == pre[after]) ++after;
+    if (after < BH && pre[after] < u1) load_q(after);
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
@@ -631,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float* state = row + w * G * kMR;
-        add_state(A, L, factor(state[D], M), *reinterpret_cast<const float4*>(state + d), state[D + 1], false);
+        add_state(A, L, factor(state[D], M), *reinterpret_cast<const float4*>(state + d), state[D + 1]);
       }
       if (whole) {
         store_out(p.out + (size_t(bh) * G + r) * D + d, A, L);
@@ -652,32 +694,45 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
       }
       __syncthreads();
       if (*flag) {
-        // a thread takes 4 dimensions of every `parts`-th partial result, kChunk loads in flight at once
-        constexpr int kChunk = 12;
+        // D / 4 lanes take a query head of every `parts`-th partial result, 4 dimensions each and kChunk loads
+        // in flight at once; lane i of them reads the i-th one's maximum and sum
+        constexpr int kLanes = D / 4, kChunk = 16;
         const float* p0 = p.part + size_t(bh + c_first) * G * kMR;
-        const int cols = G * (D / 4);
+        const int cols = G * kLanes;
         const int parts = kThreads / cols > 1 ? kThreads / cols : 1;
-        for (int e = tid; e < cols * parts; e += kThreads) {
-          const int col = e % cols, part = e / cols, r = col / (D / 4), d = 4 * (col % (D / 4));
+        const int sub = lane % kLanes;
+        for (int e = tid; e < cols * parts; e += kThreads) {  // whole groups of kLanes lanes come through together
+          const uint32_t group = kLanes == 32 ? 0xffffffffu : 0xffffu << (lane & 16);
+          const int r = e % cols / kLanes, part = e / cols, d = 4 * sub;
           float M = -INFINITY, L = 0.f;
           float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
           for (int c0 = part; c0 < np; c0 += kChunk * parts) {
             float4 v[kChunk];
-            float2 ml[kChunk];
 #pragma unroll
             for (int i = 0; i < kChunk; ++i) {
               const int c = c0 + i * parts;
-              const float* row = p0 + (size_t(c) * G + r) * kMR;
-              ml[i] = c < np ? __ldcg(reinterpret_cast<const float2*>(row + D)) : make_float2(-INFINITY, 0.f);
-              v[i] = c < np ? __ldcg(reinterpret_cast<const float4*>(row + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+              v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (c < np) v[i] = __ldcg(reinterpret_cast<const float4*>(p0 + (size_t(c) * G + r) * kMR + d));
             }
-            float m = M;
+            const int c = c0 + sub * parts;
+            float2 ml = make_float2(-INFINITY, 0.f);
+            if (sub < kChunk && c < np) ml = __ldcg(reinterpret_cast<const float2*>(p0 + (size_t(c) * G + r) * kMR + D));
+            float m = fmaxf(M, ml.x);
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) m = fmaxf(m, ml[i].x);
-            add_state(A, L, factor(M, m), A, L, true);
+            for (int o = 1; o < kLanes; o <<= 1) m = fmaxf(m, __shfl_xor_sync(group, m, o));
+            const float old = factor(M, m), f = factor(ml.x, m);
+            float l = f * ml.y;
+#pragma unroll
+            for (int o = 1; o < kLanes; o <<= 1) l += __shfl_xor_sync(group, l, o);
             M = m;
+            L = fmaf(L, old, l);
+            A.x *= old, A.y *= old, A.z *= old, A.w *= old;
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) add_state(A, L, factor(ml[i].x, m), v[i], ml[i].y, false);
+            for (int i = 0; i < kChunk; ++i) {
+              const float fi = __shfl_sync(group, f, i, kLanes);
+              A.x = fmaf(fi, v[i].x, A.x), A.y = fmaf(fi, v[i].y, A.y);
+              A.z = fmaf(fi, v[i].z, A.z), A.w = fmaf(fi, v[i].w, A.w);
+            }
           }
           if (parts == 1) {
             store_out(p.out + (size_t(bh) * G + r) * D + d, A, L);
@@ -696,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
             for (int c = 0; c < parts; ++c) M = fmaxf(M, join[(c * cols + e) * 8 + 4]);
             for (int c = 0; c < parts; ++c) {
               const float* j = join + (c * cols + e) * 8;
-              add_state(A, L, factor(j[4], M), *reinterpret_cast<const float4*>(j), j[5], false);
+              add_state(A, L, factor(j[4], M), *reinterpret_cast<const float4*>(j), j[5]);
             }
             store_out(p.out + (size_t(bh) * G + r) * D + d, A, L);
           }
@@ -704,7 +759,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNT)) kv4_decode_kernel(
       }
     }
     __syncthreads();  // merge rows free for the next head
-    rs = re;
   }
   // after a wait that gave up: leave only once every copy has landed
   if (!ok && lane == 0) {
@@ -724,12 +778,12 @@ struct DecodeLaunch {
   int sms, status;
   template <int D, int NG, int kNT>
   void launch() {
-    const size_t slot = size_t(kWarps) * kNB * Kv4<D, NG>::kRec;  // one more slot for every warp
-    const int grid = sms * ctas_per_sm(kNT);
-    const size_t fixed = fixed_smem(p.BH, p.G, D);
+    using C = Cfg<kNT>;
+    const size_t slot = size_t(C::kWarps) * kNB * Kv4<D, NG>::kRec;  // one more slot for every warp
+    const size_t fixed = fixed_smem(p.BH, p.G, D, C::kWarps);
     // As many slots as fit next to another CTA; with many heads or a large group (their prefix sums and
     // merge rows) a CTA has the SM to itself.
-    size_t room = ctas_per_sm(kNT) == 2 ? 227 * 1024 / 2 - 1024 : 227 * 1024;
+    size_t room = C::kCtas == 2 ? 227 * 1024 / 2 - 1024 : 227 * 1024;
     if (fixed + 2 * slot > room) room = 227 * 1024;
     if (fixed + 2 * slot > room) {
       status = WGKV_EINVAL;
@@ -748,8 +802,8 @@ struct DecodeLaunch {
       if (dev < 64) attr_set[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kThreads);
+    cfg.gridDim = dim3(sms * C::kCtas);
+    cfg.blockDim = dim3(C::kThreads);
     cfg.dynamicSmemBytes = fixed + p.slots * slot;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -775,7 +829,7 @@ using namespace wgkv;
 extern "C" size_t wgkv_paged_decode_kv4_workspace_size(int batch, int num_q_heads, int num_kv_heads, int head_dim) {
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || head_dim <= 0) return 0;
   const int sms = device_sms(), G = num_q_heads / num_kv_heads;
-  return workspace_bytes(int64_t(batch) * num_kv_heads, G, head_dim, (sms > 0 ? sms : 148) * ctas_per_sm(G <= 8 ? 1 : 2));
+  return workspace_bytes(int64_t(batch) * num_kv_heads, G, head_dim, (sms > 0 ? sms : 148) * (G <= 8 ? Cfg<1>::kCtas : Cfg<2>::kCtas));
 }
 
 extern "C" int wgkv_paged_decode_kv4(const uint16_t* q, const uint8_t* cache, int64_t num_pages, int page_size,
