@@ -137,7 +137,7 @@ WGKV_DEV void store_out(uint16_t* out, const float4& A, float L) {
 
 size_t fixed_smem(int BH, int G, int D, int warps) {
   return 128 + size_t(warps) * G * (D + 4) * 4 + warps * 32 * 32 + warps * kMaxSlots * 8 +
-         size_t(2 * BH + 32 * warps) * 4 + 64;
+         size_t(2 * BH + 34 * warps) * 4 + 64;
 }
 
 // Tokens of head bh that count: not below 0, not past the table.
@@ -160,8 +160,8 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
   uint64_t* bars = reinterpret_cast<uint64_t*>(join + kThreads * 8);                        // [kWarps][kMaxSlots]
   int* pre = reinterpret_cast<int*>(bars + kWarps * kMaxSlots);  // [BH] a head's first record in the line
   int* fin = pre + BH;                                           // [BH] the one behind its last
-  int* scan = fin + BH;
-  int* flag = scan + kThreads;
+  int* scan = fin + BH;                                          // [kThreads]
+  int* flag = scan + kThreads + 2 * kWarps;
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffff, tid >> 5, 0);  // the same in all lanes, so branches on it are uniform
@@ -279,10 +279,12 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
 
   // ---- this warp's records in order: of the pairs of each head's part of the segment, every kWarps-th ----
   const int upp = p.c.page >> 4;
-  int f_bh = lo, f_off = 0;  // the next batch starts at this warp's pair f_off of head f_bh's part
+  int2* from = reinterpret_cast<int2*>(scan + kThreads) + warp;  // the next batch starts at this warp's pair
+  if (lane == 0) *from = make_int2(lo, 0);                       // from->y of head from->x's part
   int f_page = 0, f_rec = -1;  // this lane's record of the batch fetched last: page id, as looked up, and place in it
   auto fetch = [&]() {         // 16 pairs, a record per lane (f_rec -1 for none); nothing here waits for the lookup
-    int h = f_bh, o = f_off + (lane >> 1);
+    __syncwarp();
+    int h = from->x, o = from->y + (lane >> 1);
     f_rec = -1;
     while (h < BH && pre[h] < u1) {
       const int first = max(pre[h], u0), last = min(fin[h], u1);
@@ -300,8 +302,8 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
       o -= c;
       ++h;
     }
-    f_bh = __shfl_sync(0xffffffff, h, 31);
-    f_off = __shfl_sync(0xffffffff, o, 31) + 1;
+    __syncwarp();
+    if (lane == 31) *from = make_int2(h, o + 1);
   };
   auto resolve = [&]() -> int {  // its place in the cache, in records
     if (f_rec < 0) return -1;
@@ -314,7 +316,6 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
   fetch();
   int batch = resolve(), used = 0;
   int slot_in = 0;
-  uint32_t flying = 0;  // slots whose copies nobody has waited for
   auto issue = [&]() {  // the next pair, if there is one, into slot slot_in
     const int at = __shfl_sync(0xffffffff, batch, used + (lane & 1));
     const uint32_t there = __ballot_sync(0xffffffff, at >= 0) & 3u;
@@ -323,7 +324,6 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
       if (lane < 2 && at >= 0)
         bulk_load(stage_base + size_t((warp * R + slot_in) * kNB + lane) * F::kRec, p.c.data + int64_t(at) * F::kRec,
                   F::kRec, &full[slot_in]);
-      flying |= 1u << slot_in;
     }
     slot_in = slot_in + 1 == R ? 0 : slot_in + 1;
     used += 2;
@@ -587,7 +587,6 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
       }
       if (!ok) return false;
       recs = ring + slot * (kNB * F::kRec);
-      flying &= ~(1u << slot);
       slot = slot + 1 == R ? 0 : slot + 1;
       ph ^= slot == 0;
       return true;
@@ -624,10 +623,7 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
       issue();
     }
 
-    // ---- this warp's state of the head into shared memory, the next head's queries on their way ----
-    int after = bh + 1;
-    while (after < BH && fin[after] == pre[after]) ++after;
-    if (after < BH && pre[after] < u1) load_q(after);
+    // ---- this warp's state of the head into shared memory ----
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
@@ -657,6 +653,10 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
           }
         }
       }
+    // the next head's queries on their way
+    int after = bh + 1;
+    while (after < BH && fin[after] == pre[after]) ++after;
+    if (after < BH && pre[after] < u1) load_q(after);
     __syncthreads();
 
     // ---- the warps' states into one: output, or this CTA's partial result ----
@@ -760,10 +760,9 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
     }
     __syncthreads();  // merge rows free for the next head
   }
-  // after a wait that gave up: leave only once every copy has landed
+  // after a wait that gave up: leave only once every copy has landed (or never came, for slots left empty)
   if (!ok && lane == 0) {
-    for (int i = 0; i < R; ++i)
-      if (flying >> i & 1u) mbar_wait(&full[i], i >= slot ? ph : ph ^ 1u);
+    for (int i = 0; i < R; ++i) mbar_wait(&full[i], i >= slot ? ph : ph ^ 1u);
   }
 }
 
