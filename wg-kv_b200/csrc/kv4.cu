@@ -29,12 +29,6 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4Pages c, Kv4Rows K, 
   const int64_t r = pos - first;
   bool valid = r >= 0 && r < n;
   if (!__any_sync(0xffffffff, valid)) return;
-  uint8_t* rec = nullptr;
-  if (valid) {
-    if (pos < 0 || pos >= int64_t(c.width) * c.page) set_error(c.err, WGKV_ERR_HEAD_CAPACITY);
-    else rec = kv4_record<D, NG>(c, bh, int(pos));
-    valid = rec != nullptr;
-  }
   const int place = int(pos) & 15;
   uint4 kr[W], vr[W];
 #pragma unroll
@@ -57,6 +51,12 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4Pages c, Kv4Rows K, 
         vr[j] = make_uint4(vw[0], vw[1], vw[2], vw[3]);
       }
     }
+  }
+  uint8_t* rec = nullptr;  // looked up while the rows arrive
+  if (valid) {
+    if (pos < 0 || pos >= int64_t(c.width) * c.page) set_error(c.err, WGKV_ERR_HEAD_CAPACITY);
+    else rec = kv4_record<D, NG>(c, bh, int(pos));
+    valid = rec != nullptr;
   }
   uint32_t words[W], pairs[NG];
   kv4_quantise<D, NG>(kr, words, pairs);

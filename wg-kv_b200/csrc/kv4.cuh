@@ -115,8 +115,10 @@ WGKV_DEV void kv4_quantise(const uint4* raw, uint32_t* words, uint32_t* pairs) {
 #pragma unroll
       for (int e = 7; e >= 0; --e) {
         const float v = e & 1 ? __uint_as_float(u[e >> 1] & 0xffff0000u) : __uint_as_float(u[e >> 1] << 16);
-        float t = __fadd_rn(__fmul_rn(__fsub_rn(v, lo[n]), inv[n]), 0.5f + 0.000244140625f);
-        t = fminf(t, 15.5f);
+        // (M - m) / scale is at most 15 (1 + 2^-8), so the bound 15.5 holds by itself.  Fusing the product
+        // and the sum changes no code: where v - m is a multiple of the scale's last bit, the quotient is
+        // 2^-17 or more (relative) away from where the code steps, 32 times fp32's roundings.
+        const float t = __fmaf_rn(__fsub_rn(v, lo[n]), inv[n], 0.5f + 0.000244140625f);
         // adding 2^23 rounding down leaves floor(t) in the low bits: 0x4b000000 + code
         w = w * 16u + __float_as_uint(__fadd_rd(t, 8388608.f));
       }
