@@ -1101,7 +1101,7 @@ def model_arm(args, rank, world, local_rank):
     n_eager = min(K, 32)
     total = P + Wu + n_eager + 2 * K + 24
     m = WgkvDecoder(shape, batch=B, window=args.window, max_tokens_per_head=total + args.window + 64,
-                    g_defer=not args.no_defer, max_positions=total, device=dev, seed=rank)
+                    g_defer=not args.no_defer, max_positions=total, device=dev, seed=rank, kv_bits=args.kv_bits)
     m.calibrate_gates()
     g = torch.Generator(device=dev)
     g.manual_seed(11 + rank)
@@ -1157,7 +1157,8 @@ def model_arm(args, rank, world, local_rank):
     wgkv.check_errors()
     glen = cache.global_lengths.double().mean().item()
     D, Hk, Ly = shape.head_dim, shape.kv_heads, shape.layers
-    kv_bytes = B * Ly * Hk * (glen + min(args.window, P)) * 2 * D * 2
+    row_bytes = wgkv.kv4_row_bytes(D, m.config.kv_cache_group) if args.kv_bits == 4 else 2 * D * 2
+    kv_bytes = B * Ly * Hk * (glen + min(args.window, P)) * row_bytes
     w_bytes = m.weight_bytes() - m.embed.numel() * 2
     tpot = max_over_ranks(graph_ms, dev) / K
     tpot_eager = max_over_ranks(eager_ms, dev) / n_eager
@@ -1186,7 +1187,7 @@ def model_arm(args, rank, world, local_rank):
             "data": "synthetic token ids; random-init weights",
             "config": {"workload": f"end-to-end decoder ({args.model}), TTFT + TPOT as scripts/profiling.py",
                        "model": shape.name, "batch": B, "prompt": P, "window": args.window, "page": 16,
-                       "g_defer": not args.no_defer, "admit": "Beta(2,8) per head (calibrated gate bias)",
+                       "kv_cache_bits": args.kv_bits, "g_defer": not args.no_defer, "admit": "Beta(2,8) per head (calibrated gate bias)",
                        "l2": "weights + KV larger than L2 each step, no flush"},
             "ttft_ms": ttft, "prefill_tok_s": B * P / (ttft / 1e3), "tpot_ms_graph": tpot, "tpot_ms_eager": tpot_eager,
             "breakdown_ms": {"prefill": bd_prefill, "decode_step": bd_decode},
@@ -1212,6 +1213,7 @@ def main():
     ap.add_argument("--prompt", type=int, default=32000, help="model workload: prompt length")
     ap.add_argument("--batch", type=int, default=1, help="model workload: sequences")
     ap.add_argument("--window", type=int, default=4096, help="model workload: local window")
+    ap.add_argument("--kv-bits", type=int, default=16, choices=[16, 4], help="model workload: bits of the KV pool")
     ap.add_argument("--no-defer", action="store_true", help="model workload: gate each token at decode")
     ap.add_argument("--small", action="store_true", help="reduced layer count for profiling captures")
     ap.add_argument("--no-prefill", action="store_true", help="skip the 400K prefill measurement of the default run")

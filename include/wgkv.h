@@ -74,7 +74,7 @@ WGKV_API int wgkv_version(void);
 /* Number of SMs of the current device (cached per device). <0 on error. */
 WGKV_API int wgkv_num_sms(void);
 
-/* ---- paged pool state (shared by the admission entry points) ------------ */
+/* ---- paged pool state (shared by the admission entry points; zero it before filling it in) ---- */
 /*
  * Device-resident state that the reference attaches to its DynamicCache in
  * prefill_wrapper (modeling_layers.py:1196-1288), with a batch axis added.
@@ -98,6 +98,11 @@ WGKV_API int wgkv_num_sms(void);
  *   free_ids/count   optional SnapKV free list (free_block_ids, :1262): device int32[total_blocks] and its
  *                    device length.  wgkv_snapkv_evict appends the pages it empties; wgkv_promote takes
  *                    new pages from the list's tail first (:694-709).  NULL = no free list.
+ *   kv4, kv4_group   optional 4-bit cache (wgkv_kv4_*) that holds the pages in place of k and v, which are
+ *                    then not used: (total_blocks, page, wgkv_kv4_row_bytes(head_dim, kv4_group)) uint8.
+ *                    Ring and global rows are quantised as they are written; promotion moves a row's codes.
+ *                    Attend with wgkv_paged_decode_kv4.  page % 16 == 0; not together with quest_min/max
+ *                    (bounds of bf16 keys) or free_ids (eviction scores and moves bf16 rows).  NULL = bf16.
  * The ring slot s of (layer l, batch b, head h) is pool row ((l*batch + b)*kv_heads + h)*window + s.
  */
 typedef struct wgkv_pool {
@@ -123,6 +128,8 @@ typedef struct wgkv_pool {
   uint16_t* quest_max;
   int32_t* free_ids;
   int32_t* free_count;
+  uint8_t* kv4;
+  int32_t kv4_group;
 } wgkv_pool;
 
 /* insert_pos / local_ptr value that means "read the position from pool->ring_state". */

@@ -169,3 +169,71 @@ def test_oracle_rule(group):
     t[0, :4] = 0, 15, 2.5, 7.5
     t[0, group - 1] = 15
     assert K4.quantise(t, group)[0][0, :4].tolist() == [0, 15, 3, 8]
+
+
+@needs_lib
+def test_call_by_array_checks_its_operation():
+    assert lib.wgkv_kv4_call(3, F) == EINVAL and lib.wgkv_kv4_call(0, None) == EINVAL
+    # the slot counts of the packed formats are the entry points' argument counts
+    from wgkv import kv4
+    for fmt, name in ((kv4._APPEND_SLOTS, "wgkv_kv4_append"), (kv4._READ_SLOTS, "wgkv_kv4_read"),
+                      (kv4._DECODE_SLOTS, "wgkv_paged_decode_kv4")):
+        assert fmt.size == 8 * len(lib.decls[name][1])
+    # argument checks are reached through it too
+    assert lib.wgkv_kv4_call(kv4._DECODE, kv4._DECODE_SLOTS.pack(F, F, 8, 24, 64, F, F, 4, 4, 1, 8, 2, 128, 1.0, F, F,
+                                                                 1 << 30, F, 0)) == EINVAL
+    assert lib.wgkv_stream_capture_id(None) == 0
+
+
+def _pool(**kw):
+    from wgkv.pool import WgkvPool
+    p = WgkvPool()
+    p.layers, p.batch, p.kv_heads, p.head_dim, p.window, p.page = 2, 3, 4, 128, 64, 16
+    p.max_blocks_per_head, p.max_tokens_per_head, p.total_blocks = 100, 1600, 10000
+    for n in ("block_table", "global_lengths", "local_is_global", "next_free_block", "err", "ring_state", "kv4"):
+        setattr(p, n, F)
+    p.kv4_group = 64
+    for n, x in kw.items():
+        setattr(p, n, x)
+    return p
+
+
+@needs_lib
+def test_pool_entry_points_refuse_what_a_4_bit_pool_cannot_do():
+    import ctypes
+
+    def promote(**kw):
+        p = _pool(**kw)
+        return lib.wgkv_promote(ctypes.addressof(p), 64, None)  # the position is refused last: nothing launches
+
+    assert promote() == EINVAL  # window 64: slot 64 does not exist
+    for bad in (dict(kv4_group=16), dict(head_dim=64, kv4_group=128), dict(page=8), dict(kv4=F + 8),
+                dict(quest_min=F), dict(free_ids=F, free_count=F), dict(kv4=None)):
+        p = _pool(**bad)
+        assert lib.wgkv_promote(ctypes.addressof(p), 3, None) == EINVAL, bad
+    p = _pool(quest_min=F, quest_max=F)
+    assert lib.wgkv_quest_select(ctypes.addressof(p), 0, 10, F, 0, 16, 144, F, F, 100, F, 1 << 20, None) == EINVAL
+    p = _pool(free_ids=F, free_count=F)
+    assert lib.wgkv_snapkv_evict(ctypes.addressof(p), F, 32, 16, 0.1, 0.3, 5, F, 1 << 30, None) == EINVAL
+
+
+def test_pool_refusals():
+    from types import SimpleNamespace
+    from wgkv.layers import _kv_group
+    kw = dict(layers=1, batch=1, kv_heads=2, head_dim=128, window=64, max_total_tokens=4096, max_tokens_per_head=1024,
+              device="cpu")
+    with pytest.raises(NotImplementedError):
+        wgkv.init_pool(SimpleNamespace(), page=16, quest=True, kv_group=64, **kw)
+    with pytest.raises(NotImplementedError):
+        wgkv.init_pool(SimpleNamespace(), page=16, snapkv_window=32, q_heads=4, kv_group=64, **kw)
+    with pytest.raises(TypeError):
+        wgkv.init_pool(SimpleNamespace(), page=16, dtype=torch.float16, kv_group=64, **kw)
+    with pytest.raises(ValueError):
+        wgkv.init_pool(SimpleNamespace(), page=8, kv_group=64, **kw)
+    with pytest.raises(ValueError):
+        wgkv.init_pool(SimpleNamespace(), page=16, kv_group=48, **kw)
+    assert _kv_group(SimpleNamespace()) is None and _kv_group(SimpleNamespace(kv_cache_bits=16)) is None
+    assert _kv_group(SimpleNamespace(kv_cache_bits=4)) == 64
+    assert _kv_group(SimpleNamespace(kv_cache_bits=4, kv_cache_group=32)) == 32
+    with pytest.raises(ValueError):
+        _kv_group(SimpleNamespace(kv_cache_bits=8))

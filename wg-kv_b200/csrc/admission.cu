@@ -18,6 +18,7 @@
 #include <string.h>
 
 #include "common.cuh"
+#include "kv4.cuh"
 #include "runtime.h"
 
 namespace wgkv {
@@ -293,18 +294,17 @@ WGKV_DEV void copy_row(uint16_t* dst, const uint16_t* src, int D, int lane_in_gr
   }
 }
 
-template <bool kVec16>
-__global__ void __launch_bounds__(kScanThreads) prefill_scatter_kernel(PoolArgs pa, int layer, int L, int n_early,
-                                                                       int n_loc, int nch, MaskView mv, RowSrc K,
-                                                                       RowSrc V, RowSrc PK, const int* counts,
-                                                                       const int* first, const int* okflag) {
-  if (!*okflag) return;
-  const wgkv_pool& P = pa.P;
-  const int Hk = P.kv_heads, BH = P.batch * Hk, D = P.head_dim;
+// The rows one CTA of a scatter kernel moves: entry e < tot of the chunk's list is the admitted token
+// list[e].x, for pool row gdst0 + e; the entries from tot to n are ring tokens, for ring slot -2 - list[e].y.
+struct ScatterRows {
+  int tot, n;
+  int64_t gdst0, ring_row0;
+};
+
+WGKV_DEV ScatterRows scatter_list(const wgkv_pool& P, int layer, int L, int n_early, int n_loc, int nch,
+                                  const MaskView& mv, const int* counts, const int* first, int2* list, int* wsum) {
+  const int Hk = P.kv_heads, BH = P.batch * Hk;
   const int bh = blockIdx.y, b = bh / Hk, h = bh - b * Hk, c = blockIdx.x;
-  __shared__ int2 list[kChunk];  // (token, -2 - ring slot for ring rows)
-  __shared__ int wsum[kScanThreads / 32];
-  __shared__ int s_n;
   const int t0 = c * kChunk + threadIdx.x * 8;
   const int ring_start = L - n_loc;  // first token that goes to the ring
   const int64_t ring_row0 = (int64_t(layer) * BH + bh) * P.window;
@@ -348,9 +348,24 @@ __global__ void __launch_bounds__(kScanThreads) prefill_scatter_kernel(PoolArgs 
       ++ri;
     }
   }
-  if (threadIdx.x == 0) s_n = tot + rtot;
   __syncthreads();
-  const int n = s_n;
+  return {tot, tot + rtot, gdst0, ring_row0};
+}
+
+template <bool kVec16>
+__global__ void __launch_bounds__(kScanThreads) prefill_scatter_kernel(PoolArgs pa, int layer, int L, int n_early,
+                                                                       int n_loc, int nch, MaskView mv, RowSrc K,
+                                                                       RowSrc V, RowSrc PK, const int* counts,
+                                                                       const int* first, const int* okflag) {
+  if (!*okflag) return;
+  const wgkv_pool& P = pa.P;
+  const int Hk = P.kv_heads, D = P.head_dim;
+  const int bh = blockIdx.y, b = bh / Hk, h = bh - b * Hk;
+  __shared__ int2 list[kChunk];  // (token, -2 - ring slot for ring rows)
+  __shared__ int wsum[kScanThreads / 32];
+  const ScatterRows rows = scatter_list(P, layer, L, n_early, n_loc, nch, mv, counts, first, list, wsum);
+  const int tot = rows.tot, n = rows.n;
+  const int64_t gdst0 = rows.gdst0, ring_row0 = rows.ring_row0;
   // copy rows: one warp-quarter (8 lanes) per row
   const int grp = threadIdx.x >> 3, gl = threadIdx.x & 7;
   if (kVec16 && D <= 128 && !(P.local_pre_key && PK.p)) {
@@ -409,6 +424,90 @@ __global__ void __launch_bounds__(kScanThreads) prefill_scatter_kernel(PoolArgs 
   }
 }
 
+// The same rows into a 4-bit pool.  Admitted rows and ring rows are two runs of consecutive pool rows; a
+// warp takes 8 rows aligned to 8 of a run (as kv4_append does), four lanes to a row.
+template <int D, int NG>
+__global__ void __launch_bounds__(kScanThreads) prefill_scatter_kv4_kernel(PoolArgs pa, int layer, int L, int n_early,
+                                                                           int n_loc, int nch, MaskView mv, RowSrc K,
+                                                                           RowSrc V, RowSrc PK, const int* counts,
+                                                                           const int* first, const int* okflag) {
+  if (!*okflag) return;
+  constexpr int W = D / 32;
+  const wgkv_pool& P = pa.P;
+  const int Hk = P.kv_heads;
+  const int bh = blockIdx.y, b = bh / Hk, h = bh - b * Hk;
+  __shared__ int2 list[kChunk];
+  __shared__ int wsum[kScanThreads / 32];
+  const ScatterRows rows = scatter_list(P, layer, L, n_early, n_loc, nch, mv, counts, first, list, wsum);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = lane & 3;
+  for (int run = 0; run < 2; ++run) {
+    const int e0 = run ? rows.tot : 0, len = run ? rows.n - rows.tot : rows.tot;
+    if (len == 0) continue;
+    const int64_t row0 = run ? rows.ring_row0 + (-2 - list[e0].y) : rows.gdst0;
+    const int lead = int(row0 & 7);
+    for (int w = warp * 8; w < lead + len; w += kScanThreads / 4) {
+      const int i = w + (lane >> 2) - lead;
+      const bool valid = i >= 0 && i < len;
+      const int64_t row = row0 + i;
+      uint4 kr[W], vr[W];
+      int64_t tok = 0;
+      if (valid) tok = list[e0 + i].x;
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        kr[j] = vr[j] = make_uint4(0, 0, 0, 0);
+        if (valid) {
+          const uint32_t* ks = reinterpret_cast<const uint32_t*>(K.p + b * K.sb + h * K.sh + tok * K.st + 32 * j + 8 * t);
+          const uint32_t* vs = reinterpret_cast<const uint32_t*>(V.p + b * V.sb + h * V.sh + tok * V.st + 32 * j + 8 * t);
+          kr[j] = make_uint4(__ldg(ks), __ldg(ks + 1), __ldg(ks + 2), __ldg(ks + 3));
+          vr[j] = make_uint4(__ldg(vs), __ldg(vs + 1), __ldg(vs + 2), __ldg(vs + 3));
+        }
+      }
+      uint8_t* rec = P.kv4 + (row >> 4) * Kv4<D, NG>::kRec;  // a page is whole records
+      const int place = int(row & 15);
+      uint32_t words[W], pairs[NG];
+      kv4_quantise<D, NG>(kr, words, pairs);
+      if (valid) kv4_store_k<D, NG>(rec, place, t, words, pairs);
+      kv4_quantise<D, NG>(vr, words, pairs);
+      const bool both = __shfl_xor_sync(0xffffffff, int(valid), 4) && valid;
+      kv4_store_v<D, NG>(rec, place, t, words, pairs, valid, both);
+      if (run && valid && P.local_pre_key && PK.p)
+        copy_row<false>(P.local_pre_key + row * D, PK.p + b * PK.sb + h * PK.sh + tok * PK.st, D, t, 4);
+    }
+  }
+}
+
+struct ScatterKv4Launch {
+  dim3 grid;
+  cudaStream_t stream;
+  PoolArgs pa;
+  int layer, L, n_early, n_loc, nch;
+  MaskView mv;
+  RowSrc K, V, PK;
+  const int *counts, *first, *okflag;
+  template <int D, int NG>
+  void run() {
+    prefill_scatter_kv4_kernel<D, NG><<<grid, kScanThreads, 0, stream>>>(pa, layer, L, n_early, n_loc, nch, mv, K, V,
+                                                                         PK, counts, first, okflag);
+  }
+};
+
+// One warp stores a new token's K and V (bf16 rows, 4-byte aligned) as pool row `row` of a 4-bit pool.
+struct PutRowKv4 {
+  uint8_t* kv4;
+  int64_t row;
+  const uint16_t *k, *v;
+  template <int D, int NG>
+  WGKV_DEV void run() const {
+    kv4_put_row<D, NG>(kv4 + (row >> 4) * Kv4<D, NG>::kRec, int(row & 15), k, v);
+  }
+};
+
+// Not inlined: five instances in kernels that are tuned for the bf16 pool.
+__device__ __noinline__ void put_row_kv4(uint8_t* kv4, int D, int group, int64_t row, const uint16_t* k,
+                                         const uint16_t* v) {
+  kv4_dispatch(D, group, PutRowKv4{kv4, row, k, v});
+}
+
 // QUEST key bounds of the global pages a prefill just filled (:1333-1347): one warp per page,
 // lanes over the head dimension.
 __global__ void __launch_bounds__(256) quest_bounds_kernel(PoolArgs pa, int layer, const int* okflag) {
@@ -459,8 +558,12 @@ __global__ void __launch_bounds__(256) decode_append_kernel(PoolArgs pa, int lay
   ring_position(P, ins, cur);
   const int b = i / Hk, h = i - b * Hk;
   const int64_t row = (int64_t(layer) * BH + i) * P.window + ins;
-  copy_row<false>(P.k + row * D, K.p + b * K.sb + h * K.sh, D, lane, 32);
-  copy_row<false>(P.v + row * D, V.p + b * V.sb + h * V.sh, D, lane, 32);
+  if (P.kv4) {
+    put_row_kv4(P.kv4, D, P.kv4_group, row, K.p + b * K.sb + h * K.sh, V.p + b * V.sb + h * V.sh);
+  } else {
+    copy_row<false>(P.k + row * D, K.p + b * K.sb + h * K.sh, D, lane, 32);
+    copy_row<false>(P.v + row * D, V.p + b * V.sb + h * V.sh, D, lane, 32);
+  }
   if (PK.p && P.local_pre_key) copy_row<false>(P.local_pre_key + row * D, PK.p + b * PK.sb + h * PK.sh, D, lane, 32);
   if (lane == 0 && cache_seqlens) cache_seqlens[i] = cur + P.global_lengths[layer * BH + i];
 }
@@ -623,6 +726,54 @@ __global__ void __launch_bounds__(256) promote_copy_kernel(PoolArgs pa, int ptr)
   }
 }
 
+// promote_copy_kernel for a 4-bit pool: a warp per head moves the row's codes and pairs as they are (no
+// second rounding), V's codes in the 2-byte pieces a token owns.
+template <int D, int NG>
+__global__ void __launch_bounds__(256) promote_copy_kv4_kernel(PoolArgs pa, int ptr) {
+  using F = Kv4<D, NG>;
+  const wgkv_pool& P = pa.P;
+  const int N = P.layers * P.batch * P.kv_heads, W = P.window, T = P.page;
+  if (ptr < 0) {
+    if (P.ring_state[0] < W) return;
+    ptr = P.ring_state[1];
+  }
+  if (P.err && (*P.err & (WGKV_ERR_HEAD_CAPACITY | WGKV_ERR_POOL_EXHAUSTED))) return;
+  const int i = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (i >= N || !P.local_is_global[int64_t(i) * W + ptr]) return;
+  const int gl = P.global_lengths[i] - 1;  // the length before this promotion
+  const int64_t dst = int64_t(P.block_table[int64_t(i) * P.max_blocks_per_head + W / T + gl / T]) * T + gl % T;
+  const int64_t src = int64_t(i) * W + ptr;
+  const int a = int(src & 15), z = int(dst & 15);
+  const uint8_t* from = P.kv4 + (src >> 4) * F::kRec;
+  uint8_t* to = P.kv4 + (dst >> 4) * F::kRec;
+  auto v_at = [](int r) { return F::kV + (r >> 3) * 4 * D + ((r & 7) >> 1) * (D / 8) + (r & 1) * 2; };
+  const int piece = (lane / (D / 32)) * 4 * (D / 8) + lane % (D / 32) * 4;  // V: chunk g, word j
+  uint32_t k = 0, kp = 0, vp = 0;
+  uint16_t v = 0;
+  if (lane < D / 8) k = reinterpret_cast<const uint32_t*>(from + a * (D / 2))[lane];
+  if (lane < D / 4) v = *reinterpret_cast<const uint16_t*>(from + v_at(a) + piece);
+  if (lane < NG) {
+    kp = reinterpret_cast<const uint32_t*>(from + F::kKP)[a * NG + lane];
+    vp = reinterpret_cast<const uint32_t*>(from + F::kVP)[a * NG + lane];
+  }
+  if (lane < D / 8) reinterpret_cast<uint32_t*>(to + z * (D / 2))[lane] = k;
+  if (lane < D / 4) *reinterpret_cast<uint16_t*>(to + v_at(z) + piece) = v;
+  if (lane < NG) {
+    reinterpret_cast<uint32_t*>(to + F::kKP)[z * NG + lane] = kp;
+    reinterpret_cast<uint32_t*>(to + F::kVP)[z * NG + lane] = vp;
+  }
+}
+
+struct PromoteKv4Launch {
+  PoolArgs pa;
+  int ptr, N;
+  cudaStream_t stream;
+  template <int D, int NG>
+  void run() {
+    promote_copy_kv4_kernel<D, NG><<<(N + 7) / 8, 256, 0, stream>>>(pa, ptr);
+  }
+};
+
 // local_length / local_ptr update after the last layer of a decode step (:1408-1413)
 __global__ void ring_advance_kernel(int32_t* rs, int W) {
   if (rs[0] < W) rs[0] += 1;
@@ -751,8 +902,12 @@ __global__ void __launch_bounds__(kDgaThreads) decode_gate_append_kernel(PoolArg
       if (j < per) xs[warp * D + lane * per + j] = x[j];
   }
   // ---- ring append (independent of the gate) ----
-  copy_row<false>(P.k + row * D, k_src, D, tid, kDgaThreads);
-  copy_row<false>(P.v + row * D, v_src, D, tid, kDgaThreads);
+  if (P.kv4) {
+    if (warp == 0) put_row_kv4(P.kv4, D, P.kv4_group, row, k_src, v_src);
+  } else {
+    copy_row<false>(P.k + row * D, k_src, D, tid, kDgaThreads);
+    copy_row<false>(P.v + row * D, v_src, D, tid, kDgaThreads);
+  }
   if (tid == 0 && cache_seqlens) cache_seqlens[i] = cur + P.global_lengths[layer * BH + i];
   if (!g.w1) return;  // deferred gating: the ring is rescored as a whole later
   __syncthreads();
@@ -797,7 +952,12 @@ __global__ void __launch_bounds__(kDgaThreads) decode_gate_append_kernel(PoolArg
 }
 
 bool pool_ok(const wgkv_pool* P) {
-  return P && P->k && P->v && P->block_table && P->global_lengths && P->local_is_global && P->next_free_block &&
+  if (!P) return false;
+  const bool rows = P->kv4 ? kv4_supported(P->head_dim, P->kv4_group) && P->page > 0 && P->page % 16 == 0 &&
+                                 (reinterpret_cast<uintptr_t>(P->kv4) & 15) == 0 && !P->quest_min && !P->quest_max &&
+                                 !P->free_ids
+                           : P->k && P->v;
+  return rows && P->block_table && P->global_lengths && P->local_is_global && P->next_free_block &&
          P->layers > 0 && P->batch > 0 && P->kv_heads > 0 && (P->head_dim == 64 || P->head_dim == 128) &&
          P->page > 0 && P->window > 0 && P->window % P->page == 0 && P->total_blocks > 0;
 }
@@ -929,10 +1089,12 @@ extern "C" int wgkv_prefill_admit(const wgkv_pool* pool, int layer, int seq_len,
                      (!pre_k || (pk_sb | pk_sh | pk_st) % 8 == 0);
   if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 3) || ((k_sb | k_sh | k_st | v_sb | v_sh | v_st) & 1))
     return WGKV_EINVAL;
-  (void)D;
   RowSrc K{k, k_sb, k_sh, k_st}, V{v, v_sb, v_sh, v_st}, PK{pre_k, pk_sb, pk_sh, pk_st};
   dim3 grid(nchunks(seq_len), BH);
-  if (vec16)
+  if (pool->kv4)
+    kv4_dispatch(D, pool->kv4_group,
+                 ScatterKv4Launch{grid, s, pa, layer, seq_len, n_early, n_loc, nch, mv, K, V, PK, counts, first, okflag});
+  else if (vec16)
     prefill_scatter_kernel<true><<<grid, kScanThreads, 0, s>>>(pa, layer, seq_len, n_early, n_loc, nch, mv, K, V, PK,
                                                                counts, first, okflag);
   else
@@ -952,7 +1114,10 @@ extern "C" int wgkv_promote(const wgkv_pool* pool, int local_ptr, void* stream) 
   promote_kernel<<<1, kPromoteThreads, 0, as_stream(stream)>>>(pa, local_ptr);
   if (cudaGetLastError() != cudaSuccess) return WGKV_ECUDA;
   const int N = pool->layers * pool->batch * pool->kv_heads;
-  promote_copy_kernel<<<(N + 31) / 32, 256, 0, as_stream(stream)>>>(pa, local_ptr);
+  if (pool->kv4)
+    kv4_dispatch(pool->head_dim, pool->kv4_group, PromoteKv4Launch{pa, local_ptr, N, as_stream(stream)});
+  else
+    promote_copy_kernel<<<(N + 31) / 32, 256, 0, as_stream(stream)>>>(pa, local_ptr);
   return cudaGetLastError() == cudaSuccess ? WGKV_OK : WGKV_ECUDA;
 }
 

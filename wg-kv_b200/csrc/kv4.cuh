@@ -224,9 +224,30 @@ WGKV_DEV float kv4_value(uint32_t code, uint32_t pair) {
   return fmaf(__uint_as_float(pair & 0xffff0000u), float(code), __uint_as_float(pair << 16));
 }
 
-// Calls f.template operator()<D, NG>() for a supported (head_dim, group); false otherwise.
+// One warp quantises the row of a new token (k and v: D bf16 each, 4-byte aligned) into place r of a
+// record: lanes 0-3 take K, lanes 4-7 V.
+template <int D, int NG>
+WGKV_DEV void kv4_put_row(uint8_t* rec, int r, const uint16_t* k, const uint16_t* v) {
+  constexpr int W = D / 32;
+  const int lane = threadIdx.x & 31, t = lane & 3;
+  uint4 raw[W];
+#pragma unroll
+  for (int j = 0; j < W; ++j) {
+    raw[j] = make_uint4(0, 0, 0, 0);
+    if (lane < 8) {
+      const uint32_t* src = reinterpret_cast<const uint32_t*>((lane < 4 ? k : v) + 32 * j + 8 * t);
+      raw[j] = make_uint4(src[0], src[1], src[2], src[3]);
+    }
+  }
+  uint32_t words[W], pairs[NG];
+  kv4_quantise<D, NG>(raw, words, pairs);
+  if (lane < 4) kv4_store_k<D, NG>(rec, r, t, words, pairs);
+  kv4_store_v<D, NG>(rec, r, t, words, pairs, lane >= 4 && lane < 8, false);
+}
+
+// Calls f.run<D, NG>() for a supported (head_dim, group); false otherwise.
 template <typename F>
-inline bool kv4_dispatch(int head_dim, int group, F&& f) {
+__host__ __device__ inline bool kv4_dispatch(int head_dim, int group, F&& f) {
   if (head_dim == 128) {
     if (group == 32) return f.template run<128, 4>(), true;
     if (group == 64) return f.template run<128, 2>(), true;

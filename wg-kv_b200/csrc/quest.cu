@@ -275,7 +275,7 @@ extern "C" size_t wgkv_quest_workspace_size(const wgkv_pool* pool) {
 extern "C" int wgkv_quest_select(const wgkv_pool* pool, int layer, int cur_local_len, const uint16_t* q, int64_t q_sb,
                                  int q_heads, int token_budget, int32_t* out_seqlens, int32_t* out_table,
                                  int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!pool || !pool->quest_min || !pool->quest_max || !q || !out_seqlens || !out_table || !workspace ||
+  if (!pool || pool->kv4 || !pool->quest_min || !pool->quest_max || !q || !out_seqlens || !out_table || !workspace ||
       layer < 0 || layer >= pool->layers || q_heads <= 0 || q_heads % pool->kv_heads ||
       q_heads / pool->kv_heads > 16)
     return WGKV_EINVAL;

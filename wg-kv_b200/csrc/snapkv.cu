@@ -469,7 +469,7 @@ extern "C" size_t wgkv_snapkv_workspace_size(const wgkv_pool* pool, int window, 
 extern "C" int wgkv_snapkv_evict(const wgkv_pool* pool, const uint16_t* queries, int window, int q_heads,
                                  float softmax_scale, double evict_ratio, int kernel_size, void* workspace,
                                  size_t workspace_bytes, void* stream) {
-  if (!pool || !pool->free_ids || !pool->free_count || !queries || !workspace || window <= 0 || q_heads <= 0 ||
+  if (!pool || pool->kv4 || !pool->free_ids || !pool->free_count || !queries || !workspace || window <= 0 || q_heads <= 0 ||
       q_heads % pool->kv_heads || kernel_size <= 0 || kernel_size % 2 == 0 || !(evict_ratio > 0.0) ||
       evict_ratio > 1.0)
     return WGKV_EINVAL;

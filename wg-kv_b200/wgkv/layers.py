@@ -12,6 +12,10 @@ Mirrors the operator surface the patched Llama/Qwen3 attention layers call
 * ``self_attn_decode_fused``: the decode step fed by raw q/k/v projection rows
   (q/k norm + RoPE fused into the gate launch)
 
+``config.kv_cache_bits = 4`` holds the pool in 4 bits (:mod:`wgkv.kv4`; ``config.kv_cache_group``
+dimensions share a scale, 64 by default): rows are quantised as admission, the ring append and
+promotion write them, decode attends over the codes, and prefill attention still reads the bf16 keys.
+
 ``self`` is the attention module (``layer_idx``, ``config``, ``head_dim``,
 ``scaling``, ``g_predictors`` and the kernel slots); ``past_key_value`` is any
 attribute holder (the HF cache object), which gets the pool attributes of
@@ -30,6 +34,7 @@ import torch
 
 from ._lib import check, lib
 from .indices import sparse_indices_into
+from .kv4 import kv4_read, paged_decode_kv4
 from .pool import RING_ON_DEVICE, init_pool, pool_ref
 from .prefill import sparse_attn_func, sparse_attn_func_pooled, sparse_attn_func_wrapper
 from .runtime import stream_ptr, workspace
@@ -37,6 +42,14 @@ from .runtime import stream_ptr, workspace
 
 def _cfg(self):
     return self.config
+
+
+def _kv_group(c):
+    """Group size of a 4-bit pool, None for a bf16 one."""
+    bits = getattr(c, "kv_cache_bits", 16)
+    if bits not in (4, 16):
+        raise ValueError(f"config.kv_cache_bits must be 16 or 4, got {bits}")
+    return getattr(c, "kv_cache_group", 64) if bits == 4 else None
 
 
 def _maybe_init(self, past_key_value, batch_size, key_states):
@@ -49,9 +62,14 @@ def _maybe_init(self, past_key_value, batch_size, key_states):
                   device=key_states.device, dtype=key_states.dtype, defer=bool(getattr(c, "g_defer", False)),
                   quest=bool(getattr(c, "use_quest", False)),
                   snapkv_window=c.snapkv_window_size if getattr(c, "snapkv_enabled", False) else None,
-                  q_heads=getattr(c, "num_attention_heads", None))
+                  q_heads=getattr(c, "num_attention_heads", None), kv_group=_kv_group(c))
     elif self.layer_idx == 0:
         raise AssertionError("prefill on an initialised cache (the reference asserts the same, :1197)")
+
+
+def _kv4(cache):
+    """The pool's pages if it is held in 4 bits, else None."""
+    return getattr(cache, "block_pool_kv4", None)
 
 
 def _device_ring(cache):
@@ -88,7 +106,7 @@ def prefill_wrapper(self, past_key_value, query_states, pre_key, key_states, val
     check(st, "wgkv_prefill_admit")
     past_key_value.local_length = min(L, W)
     bc, bo, cc, ci = sparse_indices_into(g_mask, W, L, 64)
-    if self.prefill_kernel in (sparse_attn_func_wrapper, sparse_attn_func):
+    if _kv4(past_key_value) is None and self.prefill_kernel in (sparse_attn_func_wrapper, sparse_attn_func):
         # fast path: the admitted columns were just packed into contiguous pool pages
         return sparse_attn_func_pooled(query_states.transpose(1, 2), key_states.transpose(1, 2),
                                        value_states.transpose(1, 2), bc, bo, cc, ci, past_key_value.block_pool_k,
@@ -114,6 +132,16 @@ def refresh_local_is_global(self, past_key_value, device):
     c = _cfg(self)
     l = self.layer_idx
     B, Hk, W, D = past_key_value.wgkv_batch, c.num_key_value_heads, c.local_window_size, self.head_dim
+    kv4 = _kv4(past_key_value)
+    if kv4 is not None:
+        ring_k = ring_v = None
+        if {"post_k", "v"} & set(self.g_predictors.g_inputs):  # the gate sees the ring's keys as they are held
+            ring_k, ring_v = kv4_read(kv4, None,
+                                      torch.full((B, Hk), W, dtype=torch.int32, device=device),
+                                      past_key_value.block_table[l][:, :, :W // c.block_size], W)
+        self.g_predictors.admit(past_key_value.local_pre_key[l], ring_k, ring_v, c.g_threshold,
+                                past_key_value.local_is_global[l])
+        return
     n_ring = c.num_hidden_layers * B * Hk * W
     ring_k = past_key_value.block_pool_k[:n_ring].view(c.num_hidden_layers, B, Hk, W, D)[l]
     ring_v = past_key_value.block_pool_v[:n_ring].view(c.num_hidden_layers, B, Hk, W, D)[l]
@@ -154,6 +182,11 @@ def decode_wrapper(self, past_key_value, query_states, pre_key, key_states, valu
             past_key_value.local_length = cur
         else:
             past_key_value.local_ptr = (past_key_value.local_ptr + 1) % W
+    kv4 = _kv4(past_key_value)
+    if kv4 is not None:
+        q = query_states.transpose(1, 2)
+        return self.decode_kernel_executor(lambda: paged_decode_kv4(q, kv4, past_key_value.cache_seqlens,
+                                                                    past_key_value.block_table[l], self.scaling))
     T = c.block_size
     k_cache = past_key_value.block_pool_k.view(past_key_value.total_blocks, T, self.head_dim)
     v_cache = past_key_value.block_pool_v.view(past_key_value.total_blocks, T, self.head_dim)

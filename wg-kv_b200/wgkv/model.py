@@ -122,7 +122,7 @@ class WgkvDecoder:
 
     def __init__(self, shape: DecoderShape, *, batch=1, window=4096, page=16, max_tokens_per_head=33000,
                  avg_tokens_per_head=None, g_defer=True, threshold=0.5, gate_inner=64, admit=(2.0, 8.0),
-                 max_positions=None, device="cuda", seed=0, fused=True):
+                 max_positions=None, device="cuda", seed=0, fused=True, kv_bits=16, kv_group=64):
         self.s = s = shape
         self.fused = fused
         self.B = batch
@@ -145,7 +145,8 @@ class WgkvDecoder:
         self.config = SimpleNamespace(
             num_hidden_layers=s.layers, num_key_value_heads=Hk, num_attention_heads=Hq, head_dim=D,
             hidden_size=Hd, block_size=page, local_window_size=window, g_defer=g_defer, g_threshold=threshold,
-            max_tokens_per_head=max_tokens_per_head, max_total_tokens=per_head * s.layers * Hk * batch + 2 * page)
+            max_tokens_per_head=max_tokens_per_head, max_total_tokens=per_head * s.layers * Hk * batch + 2 * page,
+            kv_cache_bits=kv_bits, kv_cache_group=kv_group)  # 4: the pool is held in 4 bits
         from . import attach
         rng = np.random.default_rng(seed + 1)
         self.admit_rates = rng.beta(admit[0], admit[1], (s.layers, Hk))

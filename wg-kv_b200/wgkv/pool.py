@@ -15,6 +15,7 @@ import ctypes
 
 import torch
 
+from .kv4 import kv4_alloc
 from .runtime import err_word
 
 
@@ -43,12 +44,23 @@ class WgkvPool(ctypes.Structure):
         ("quest_max", ctypes.c_void_p),
         ("free_ids", ctypes.c_void_p),
         ("free_count", ctypes.c_void_p),
+        ("kv4", ctypes.c_void_p),
+        ("kv4_group", ctypes.c_int32),
     ]
 
 
 def init_pool(cache, *, layers, batch, kv_heads, head_dim, window, page, max_total_tokens, max_tokens_per_head,
-              device, dtype=torch.bfloat16, defer=False, quest=False, snapkv_window=None, q_heads=None):
-    """Allocate the pool on ``cache`` (any attribute holder), as prefill_wrapper does at layer 0."""
+              device, dtype=torch.bfloat16, defer=False, quest=False, snapkv_window=None, q_heads=None,
+              kv_group=None):
+    """Allocate the pool on ``cache`` (any attribute holder), as prefill_wrapper does at layer 0.
+
+    ``kv_group`` (32, 64 or 128): hold the pages in 4 bits with a scale per that many dimensions
+    (``cache.block_pool_kv4``, see :mod:`wgkv.kv4`); ``block_pool_k`` / ``block_pool_v`` are then None."""
+    if kv_group is not None:
+        if quest or snapkv_window:
+            raise NotImplementedError("QUEST and SnapKV score bf16 keys; they do not run on a 4-bit pool")
+        if dtype != torch.bfloat16:
+            raise TypeError("a 4-bit pool takes bf16 keys and values")
     assert window % page == 0, "local_window_size must be a multiple of block_size"
     local_pages = window // page
     total_local = layers * batch * kv_heads * local_pages
@@ -62,8 +74,13 @@ def init_pool(cache, *, layers, batch, kv_heads, head_dim, window, page, max_tot
                                    device=dev)
     cache.block_table[..., :local_pages] = torch.arange(total_local, dtype=torch.int32, device=dev).view(
         layers, batch, kv_heads, local_pages)
-    cache.block_pool_k = torch.empty(total_blocks * page, head_dim, dtype=dtype, device=dev)
-    cache.block_pool_v = torch.empty(total_blocks * page, head_dim, dtype=dtype, device=dev)
+    if kv_group is None:
+        cache.block_pool_k = torch.empty(total_blocks * page, head_dim, dtype=dtype, device=dev)
+        cache.block_pool_v = torch.empty(total_blocks * page, head_dim, dtype=dtype, device=dev)
+        cache.block_pool_kv4 = None
+    else:
+        cache.block_pool_k = cache.block_pool_v = None
+        cache.block_pool_kv4 = kv4_alloc(total_blocks, page, head_dim, kv_group, dev)
     cache.local_is_global = torch.zeros(layers, batch, kv_heads, window, dtype=torch.uint8, device=dev)
     cache.global_lengths = torch.zeros(layers, batch, kv_heads, dtype=torch.int32, device=dev)
     cache.local_pre_key = (torch.empty(layers, batch, kv_heads, window, head_dim, dtype=dtype, device=dev)
@@ -91,8 +108,12 @@ def init_pool(cache, *, layers, batch, kv_heads, head_dim, window, page, max_tot
         cache.quest_block_key_min = torch.zeros(total_blocks, head_dim, dtype=dtype, device=dev)
         cache.quest_block_key_max = torch.zeros(total_blocks, head_dim, dtype=dtype, device=dev)
     s = WgkvPool()
-    s.k = cache.block_pool_k.data_ptr()
-    s.v = cache.block_pool_v.data_ptr()
+    if kv_group is None:
+        s.k = cache.block_pool_k.data_ptr()
+        s.v = cache.block_pool_v.data_ptr()
+    else:
+        s.kv4 = cache.block_pool_kv4.data_ptr()
+        s.kv4_group = kv_group
     s.block_table = cache.block_table.data_ptr()
     s.global_lengths = cache.global_lengths.data_ptr()
     s.local_is_global = cache.local_is_global.data_ptr()
