@@ -83,6 +83,24 @@ WGKV_DEV void mma_f16_16816_first(float* d, uint32_t a0, uint32_t a1, uint32_t a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
+// Two fp32 values in a register pair, added and multiplied by one instruction each (same roundings).
+WGKV_DEV uint64_t f2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+WGKV_DEV float f2_get(uint64_t v, int i) { return __uint_as_float(uint32_t(v >> (32 * i))); }
+WGKV_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+WGKV_DEV uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 WGKV_DEV uint32_t pack_f16x2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -393,13 +411,13 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
       }
     }
 
-    float acc[kNT][2 * W][4];     // O^T: m-tile, (dimension g: heads 2 t4, + 1; dimension g + 8: the same)
+    uint64_t acc[kNT][2 * W][2];  // O^T: m-tile, row g and g + 8, heads 2 t4 and 2 t4 + 1 as an fp32 pair
     float um[kNT][NG][2];         // sum of p m_v over this lane's tokens
     float mx[kNT][2], l[kNT][2];
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
-      for (int m = 0; m < 2 * W; ++m) acc[nt][m][0] = acc[nt][m][1] = acc[nt][m][2] = acc[nt][m][3] = 0.f;
+      for (int m = 0; m < 2 * W; ++m) acc[nt][m][0] = acc[nt][m][1] = 0;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         mx[nt][c] = 0.f;
@@ -492,7 +510,8 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
       for (int nt = 0; nt < kNT; ++nt) move |= fmaxf(top[nt][0], top[nt][1]) > 8388608.f + 127.f + 8.f;
       if (__any_sync(0xffffffff, move)) {
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt)
+        for (int nt = 0; nt < kNT; ++nt) {
+          float fac[2];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             float m = top[nt][c];
@@ -512,12 +531,15 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
             l[nt][c] *= f;
 #pragma unroll
             for (int n2 = 0; n2 < NG; ++n2) um[nt][n2][c] *= f;
-#pragma unroll
-            for (int m2 = 0; m2 < 2 * W; ++m2) {
-              acc[nt][m2][c] *= f;
-              acc[nt][m2][2 + c] *= f;
-            }
+            fac[c] = f;
           }
+          const uint64_t both = f2(fac[0], fac[1]);
+#pragma unroll
+          for (int m2 = 0; m2 < 2 * W; ++m2) {
+            acc[nt][m2][0] = mul2(acc[nt][m2][0], both);
+            acc[nt][m2][1] = mul2(acc[nt][m2][1], both);
+          }
+        }
         first = false;
       }
     };
@@ -565,9 +587,15 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
             const uint32_t a8 = __byte_perm(v0[j], 0, 0x4341), b8 = __byte_perm(v1[j], 0, 0x4341);
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt) {
-              mma_f16_16816(acc[nt][2 * j], a, a8, b, b8, pb[nt][0], pb[nt][1]);
-              mma_f16_16816(acc[nt][2 * j + 1], a & 0x00f000f0u, a8 & 0x00f000f0u, b & 0x00f000f0u, b8 & 0x00f000f0u,
-                            pb[nt][0], pb[nt][1]);
+              float d[4], e[4];
+              mma_f16_16816_first(d, a, a8, b, b8, pb[nt][0], pb[nt][1]);
+              mma_f16_16816_first(e, a & 0x00f000f0u, a8 & 0x00f000f0u, b & 0x00f000f0u, b8 & 0x00f000f0u, pb[nt][0],
+                                  pb[nt][1]);
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                acc[nt][2 * j][c] = add2(acc[nt][2 * j][c], f2(d[2 * c], d[2 * c + 1]));
+                acc[nt][2 * j + 1][c] = add2(acc[nt][2 * j + 1][c], f2(e[2 * c], e[2 * c + 1]));
+              }
             }
           }
         }
@@ -640,11 +668,13 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
 #pragma unroll
           for (int j = 0; j < W; ++j) {
             const float m = um[nt][j * NG / W][c];
+            const float e0 = f2_get(acc[nt][2 * j][0], c), o0 = f2_get(acc[nt][2 * j + 1][0], c);
+            const float e1 = f2_get(acc[nt][2 * j][1], c), o1 = f2_get(acc[nt][2 * j + 1][1], c);
             float4 v;
-            v.x = fmaf(acc[nt][2 * j][c] - acc[nt][2 * j + 1][c], 16777216.f, m);
-            v.y = fmaf(acc[nt][2 * j + 1][c], 1048576.f, m);
-            v.z = fmaf(acc[nt][2 * j][2 + c] - acc[nt][2 * j + 1][2 + c], 16777216.f, m);
-            v.w = fmaf(acc[nt][2 * j + 1][2 + c], 1048576.f, m);
+            v.x = fmaf(e0 - o0, 16777216.f, m);
+            v.y = fmaf(o0, 1048576.f, m);
+            v.z = fmaf(e1 - o1, 16777216.f, m);
+            v.w = fmaf(o1, 1048576.f, m);
             *reinterpret_cast<float4*>(row + 32 * j + 4 * g) = v;
           }
           if (g == 0) {
