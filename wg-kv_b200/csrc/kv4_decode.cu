@@ -20,6 +20,10 @@
 //   x + exponent(s_v), not over x, so that the weights, not the probabilities, are near 1 however V's
 //   scale differs between tokens; it moves only when a weight would pass 2^9.  Exponents below -40 count
 //   as -40.  Sums of p and p m_v stay fp32.
+// * The tensor cores' fp32 accumulation truncates.  Sums of codes, all positive, lose up to 2^-23 of
+//   themselves with every record added, and V's that cancel (any long, flat softmax) leave a result
+//   hundreds of times smaller than the sums: 8e-3 of it was lost at 28K tokens.  So each record's products
+//   start from zero and join O^T by paired fp32 additions, which round to nearest.
 // * S^T's accumulators hold a token per lane row, P^T's fragment a head per lane row: movmatrix turns the
 //   packed weights, one per 8x8 block.
 //
@@ -136,6 +140,26 @@ WGKV_DEV void lds_words(uint32_t* w, uint32_t a) {
     asm("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(a) : "memory");
 }
 
+// One look at a barrier's phase; most pairs have arrived when they are asked for.
+WGKV_DEV bool mbar_done(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n"
+      " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done;
+}
+
+// The rest of a wait, with its limit; once one of a CTA has run into it the others do not wait at all.
+__device__ __noinline__ void wait_longer(uint64_t* bar, uint32_t parity, volatile int* gave_up, int* err) {
+  if (*gave_up || mbar_wait(bar, parity)) return;
+  *gave_up = 1;
+  set_error(err, WGKV_ERR_TIMEOUT);
+}
+
 template <int D>
 __host__ __device__ constexpr int merge_row() { return D + 4; }  // D values, maximum, sum; rows 16 bytes apart mod 128
 
@@ -180,13 +204,15 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
   int* fin = pre + BH;                                           // [BH] the one behind its last
   int* scan = fin + BH;                                          // [kThreads]
   int* flag = scan + kThreads + 2 * kWarps;
+  volatile int* gave_up = flag + 1;  // a wait of this CTA ran into its limit
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffff, tid >> 5, 0);  // the same in all lanes, so branches on it are uniform
   const uint32_t ring = smem_u32(stage_base) + warp * R * kNB * F::kRec;
   uint64_t* full = bars + warp * kMaxSlots;
-  if (lane < R) mbar_init(&full[lane], 1);
+  if (lane < R) mbar_init(&full[lane], kNB);
   fence_barrier_init();
+  *gave_up = 0;
   griddep_wait();  // lengths, tables and rows may come from the launch just before
   griddep_launch();
 
@@ -334,14 +360,16 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
   fetch();
   int batch = resolve(), used = 0;
   int slot_in = 0;
-  auto issue = [&]() {  // the next pair, if there is one, into slot slot_in
+  auto issue = [&]() {  // the next pair into slot slot_in
     const int at = __shfl_sync(0xffffffff, batch, used + (lane & 1));
-    const uint32_t there = __ballot_sync(0xffffffff, at >= 0) & 3u;
-    if (there) {
-      if (lane == 0) mbar_arrive_expect_tx(&full[slot_in], there == 3u ? 2 * F::kRec : F::kRec);
-      if (lane < 2 && at >= 0)
+    if (lane < kNB && !*gave_up) {  // a slot whose copies never came is not armed again
+      if (at >= 0) {
+        mbar_arrive_expect_tx(&full[slot_in], F::kRec);
         bulk_load(stage_base + size_t((warp * R + slot_in) * kNB + lane) * F::kRec, p.c.data + int64_t(at) * F::kRec,
                   F::kRec, &full[slot_in]);
+      } else {
+        mbar_arrive(&full[slot_in]);  // a pair of one record, or none
+      }
     }
     slot_in = slot_in + 1 == R ? 0 : slot_in + 1;
     used += 2;
@@ -356,7 +384,6 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
 
   int slot = 0;       // the next pair's
   uint32_t ph = 0;
-  bool ok = true;
   for (int bh = lo; bh < BH && pre[bh] < u1; ++bh) {
     const int hs = pre[bh], he = fin[bh];
     const int rs = max(hs, u0), re = min(he, u1);
@@ -608,24 +635,21 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
     const int pairs = (re - rs + 1) >> 1;
     const int mine = (pairs - warp + kWarps - 1) / kWarps;                   // this warp's
     const int whole_pairs = mine - (mine > 0 && (pairs - 1) % kWarps == warp);
-    auto arrived = [&](uint32_t& recs) -> bool {  // the next pair's slot, its copies landed
-      if (ok && !mbar_wait(&full[slot], ph)) {    // the head's result is lost; the counters below still come out right
-        set_error(p.c.err, WGKV_ERR_TIMEOUT);
-        ok = false;
-      }
-      if (!ok) return false;
-      recs = ring + slot * (kNB * F::kRec);
+    auto arrived = [&]() -> uint32_t {  // the next pair's slot, its copies landed
+      if (!mbar_done(&full[slot], ph)) wait_longer(&full[slot], ph, gave_up, p.c.err);
+      const uint32_t recs = ring + slot * (kNB * F::kRec);
       slot = slot + 1 == R ? 0 : slot + 1;
       ph ^= slot == 0;
-      return true;
+      return recs;
     };
     Scores x;
     float top[kNT][2];
-    uint32_t now = 0, next = 0;
-    if (whole_pairs > 0 && arrived(now)) {
+    if (whole_pairs > 0) {
+      uint32_t now = arrived();
       scores(now, Whole<true>(), kNB, 0, x, top);
       settle(x, top);
-      for (int i = 1; i < whole_pairs && arrived(next); ++i) {
+      for (int i = 1; i < whole_pairs; ++i) {
+        const uint32_t next = arrived();
         Scores y;
         scores(next, Whole<true>(), kNB, 0, y, top);
         weigh(now, Whole<true>(), kNB, 0, x);
@@ -635,13 +659,12 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
         x = y;
         now = next;
       }
-      if (ok) {
-        weigh(now, Whole<true>(), kNB, 0, x);
-        __syncwarp();
-        issue();
-      }
+      weigh(now, Whole<true>(), kNB, 0, x);
+      __syncwarp();
+      issue();
     }
-    if (mine > whole_pairs && arrived(now)) {
+    if (mine > whole_pairs) {
+      const uint32_t now = arrived();
       const int u = rs + 2 * (pairs - 1);
       const int nb = min(kNB, re - u), left = head_len(p, bh) - (u - pre[bh]) * 16;
       scores(now, Whole<false>(), nb, left, x, top);
@@ -790,8 +813,9 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
     }
     __syncthreads();  // merge rows free for the next head
   }
-  // after a wait that gave up: leave only once every copy has landed (or never came, for slots left empty)
-  if (!ok && lane == 0) {
+  // after a wait that gave up (the results are lost, the counters came out right): leave only once every
+  // copy has landed, or never came
+  if (*gave_up && lane == 0) {
     for (int i = 0; i < R; ++i) mbar_wait(&full[i], i >= slot ? ph : ph ^ 1u);
   }
 }
