@@ -187,18 +187,21 @@ WGKV_DEV int head_len(const Kv4DecodeParams& p, int bh) {
   return min(max(__ldg(p.seqlens + bh), 0), p.c.width * p.c.page);
 }
 
-// kNT: 8-head tiles of query heads (G <= 8: 1, G <= 16: 2).
-template <int D, int NG, int kNT>
+// kNT: 8-head tiles of query heads (G <= 8: 1, G <= 16: 2).  kPack: records whose scores share the 8
+// columns of a tile (G <= 4: 2).
+template <int D, int NG, int kNT, int kPack>
 __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decode_kernel(Kv4DecodeParams p) {
   using F = Kv4<D, NG>;
   constexpr int kWarps = Cfg<kNT>::kWarps, kThreads = Cfg<kNT>::kThreads;
+  constexpr int kSets = kNB / kPack;        // sets of columns a pair of records fills
+  static_assert(kPack == 1 || (kPack == 2 && kNT == 1), "two records share one tile of columns");
   constexpr int W = D / 32;
   constexpr int kMR = merge_row<D>();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stage_base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
   const int R = p.slots, G = p.G, BH = p.BH;
   float* merge = reinterpret_cast<float*>(stage_base + size_t(kWarps) * R * kNB * F::kRec);  // [kWarps][G][kMR]
-  float* join = merge + kWarps * G * kMR;                                                   // [kThreads][8]
+  float* join = merge + kWarps * G * kMR;                                                  // [kThreads][8]
   uint64_t* bars = reinterpret_cast<uint64_t*>(join + kThreads * 8);                        // [kWarps][kMaxSlots]
   int* pre = reinterpret_cast<int*>(bars + kWarps * kMaxSlots);  // [BH] a head's first record in the line
   int* fin = pre + BH;                                           // [BH] the one behind its last
@@ -306,13 +309,16 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
 
   // the queries of the first head are on their way while its pages are looked up
   const int g = lane >> 2, t4 = lane & 3;
+  // kPack = 2: columns 0-3 are the heads for the first record of a pair, columns 4-7 for the second
+  const int half = kPack == 2 ? t4 >> 1 : 0;
+  const uint32_t own[2] = {g < 4 ? 0xffffffffu : 0u, g < 4 ? 0u : 0xffffffffu};
   uint4 raw_q[kNT][W];
   auto load_q = [&](int bh) {
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
       for (int j = 0; j < W; ++j) {
-        const int head = nt * 8 + g;
+        const int head = kPack == 2 ? g & 3 : nt * 8 + g;
         raw_q[nt][j] = make_uint4(0, 0, 0, 0);
         if (head < G)
           raw_q[nt][j] = __ldg(reinterpret_cast<const uint4*>(p.q + (size_t(bh) * G + head) * D + 32 * j + 8 * t4));
@@ -456,7 +462,7 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
 
     bool first = true;  // no reference yet
     struct Scores {
-      float v[kNB][kNT][4];
+      float v[kSets][kNT][4];
     };
     // Scores of a pair of records relative to the reference, and a bound of their weights.  kAll: both are
     // there and every token counts, so that nothing branches.
@@ -465,31 +471,38 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < kNB; ++i) {
+      for (int i = 0; i < kSets; ++i) {
         if (!kAll && i >= nb) continue;
-        const uint32_t rec = recs + i * F::kRec;
-        uint32_t k0[W], k1[W], kp0[NG], kp1[NG];
-        lds_words<W>(k0, rec + lane * (D / 8));
-        lds_words<W>(k1, rec + 4 * D + lane * (D / 8));
+        uint32_t k0[kPack][W], k1[kPack][W], kp0[NG], kp1[NG];
+#pragma unroll
+        for (int r = 0; r < kPack; ++r) {
+          lds_words<W>(k0[r], recs + (i + r) * F::kRec + lane * (D / 8));
+          lds_words<W>(k1[r], recs + (i + r) * F::kRec + 4 * D + lane * (D / 8));
+        }
+        const int mine = kPack == 2 ? half : i;  // the record whose tokens this lane's columns are about
+        const uint32_t rec = recs + mine * F::kRec;
         lds_words<NG>(kp0, rec + F::kKP + g * 4 * NG);
         lds_words<NG>(kp1, rec + F::kKP + (g + 8) * 4 * NG);
         float t[kNT][4], o[kNT][4];
 #pragma unroll
         for (int n2 = 0; n2 < NG; ++n2) {
-          float d[kNT][4];
+          float d[kPack][kNT][4];
 #pragma unroll
           for (int j = n2 * (W / NG); j < (n2 + 1) * (W / NG); ++j) {
-            const uint32_t a = k0[j], b = k1[j], a8 = a >> 8, b8 = b >> 8;
 #pragma unroll
-            for (int nt = 0; nt < kNT; ++nt) {
-              if (j == n2 * (W / NG))
-                mma_f16_16816_first(d[nt], a & 0x000f000fu, b & 0x000f000fu, a8 & 0x000f000fu, b8 & 0x000f000fu,
-                                    qf[nt][j][0], qf[nt][j][1]);
-              else
-                mma_f16_16816(d[nt], a & 0x000f000fu, b & 0x000f000fu, a8 & 0x000f000fu, b8 & 0x000f000fu,
-                              qf[nt][j][0], qf[nt][j][1]);
-              mma_f16_16816(d[nt], a & 0x00f000f0u, b & 0x00f000f0u, a8 & 0x00f000f0u, b8 & 0x00f000f0u,
-                            qf[nt][j][2], qf[nt][j][3]);
+            for (int r = 0; r < kPack; ++r) {
+              const uint32_t a = k0[r][j], b = k1[r][j], a8 = a >> 8, b8 = b >> 8;
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt) {
+                if (j == n2 * (W / NG))
+                  mma_f16_16816_first(d[r][nt], a & 0x000f000fu, b & 0x000f000fu, a8 & 0x000f000fu, b8 & 0x000f000fu,
+                                      qf[nt][j][0], qf[nt][j][1]);
+                else
+                  mma_f16_16816(d[r][nt], a & 0x000f000fu, b & 0x000f000fu, a8 & 0x000f000fu, b8 & 0x000f000fu,
+                                qf[nt][j][0], qf[nt][j][1]);
+                mma_f16_16816(d[r][nt], a & 0x00f000f0u, b & 0x00f000f0u, a8 & 0x00f000f0u, b8 & 0x00f000f0u,
+                              qf[nt][j][2], qf[nt][j][3]);
+              }
             }
           }
           const float s0 = __uint_as_float(kp0[n2] & 0xffff0000u), m0 = __uint_as_float(kp0[n2] << 16);
@@ -498,8 +511,10 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
           for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              t[nt][c] = n2 ? fmaf(s0, d[nt][c], t[nt][c]) : s0 * d[nt][c];
-              t[nt][2 + c] = n2 ? fmaf(s1, d[nt][2 + c], t[nt][2 + c]) : s1 * d[nt][2 + c];
+              const float d0 = kPack == 2 && half ? d[kPack - 1][nt][c] : d[0][nt][c];
+              const float d1 = kPack == 2 && half ? d[kPack - 1][nt][2 + c] : d[0][nt][2 + c];
+              t[nt][c] = n2 ? fmaf(s0, d0, t[nt][c]) : s0 * d0;
+              t[nt][2 + c] = n2 ? fmaf(s1, d1, t[nt][2 + c]) : s1 * d1;
               o[nt][c] = fmaf(m0, qs[nt][n2][c], n2 ? o[nt][c] : -mx[nt][c]);
               o[nt][2 + c] = fmaf(m1, qs[nt][n2][c], n2 ? o[nt][2 + c] : -mx[nt][c]);
             }
@@ -517,7 +532,7 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
           v1 = max(v1, vp1[n2]);
         }
         const float e0 = __uint_as_float(0x4b000000u | v0 >> 23), e1 = __uint_as_float(0x4b000000u | v1 >> 23);
-        const int valid = left - 16 * i;
+        const int valid = left - 16 * mine;
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
@@ -551,7 +566,7 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
             const float f = first ? 0.f : exp2_approx(-by);
             mx[nt][c] += by;
 #pragma unroll
-            for (int i = 0; i < kNB; ++i) {
+            for (int i = 0; i < kSets; ++i) {
               x.v[i][nt][c] -= by;
               x.v[i][nt][2 + c] -= by;
             }
@@ -574,15 +589,19 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
     auto weigh = [&](uint32_t recs, auto all, int nb, int left, const Scores& x) {
       constexpr bool kAll = decltype(all)::value;
 #pragma unroll
-      for (int i = 0; i < kNB; ++i) {
+      for (int i = 0; i < kSets; ++i) {
         if (!kAll && i >= nb) continue;
-        const uint32_t rec = recs + i * F::kRec;
-        const int valid = left - 16 * i;
-        uint32_t v0[W], v1[W], vp0[NG], vp1[NG];
-        lds_words<W>(v0, rec + F::kV + lane * (D / 8));
-        lds_words<W>(v1, rec + F::kV + 4 * D + lane * (D / 8));
+        const int mine = kPack == 2 ? half : i;
+        const uint32_t rec = recs + mine * F::kRec;
+        const int valid = left - 16 * mine;
+        uint32_t v0[kPack][W], v1[kPack][W], vp0[NG], vp1[NG];
         lds_words<NG>(vp0, rec + F::kVP + g * 4 * NG);
         lds_words<NG>(vp1, rec + F::kVP + (g + 8) * 4 * NG);
+#pragma unroll
+        for (int r = 0; r < kPack; ++r) {
+          lds_words<W>(v0[r], recs + (i + r) * F::kRec + F::kV + lane * (D / 8));
+          lds_words<W>(v1[r], recs + (i + r) * F::kRec + F::kV + 4 * D + lane * (D / 8));
+        }
         float pr[kNT][4];
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) {
@@ -599,31 +618,46 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
           }
           const float s0 = __uint_as_float(vp0[n2] & 0xffff0000u), m0 = __uint_as_float(vp0[n2] << 16);
           const float s1 = __uint_as_float(vp1[n2] & 0xffff0000u), m1 = __uint_as_float(vp1[n2] << 16);
-          uint32_t pb[kNT][2];
+          uint32_t pb[kPack][kNT][2];
 #pragma unroll
           for (int nt = 0; nt < kNT; ++nt) {
             um[nt][n2][0] = fmaf(pr[nt][0], m0, fmaf(pr[nt][2], m1, um[nt][n2][0]));
             um[nt][n2][1] = fmaf(pr[nt][1], m0, fmaf(pr[nt][3], m1, um[nt][n2][1]));
-            pb[nt][0] = movmatrix_trans(pack_f16x2(pr[nt][0] * s0, pr[nt][1] * s0));
-            pb[nt][1] = movmatrix_trans(pack_f16x2(pr[nt][2] * s1, pr[nt][3] * s1));
+            const uint32_t w0 = movmatrix_trans(pack_f16x2(pr[nt][0] * s0, pr[nt][1] * s0));
+            const uint32_t w1 = movmatrix_trans(pack_f16x2(pr[nt][2] * s1, pr[nt][3] * s1));
+#pragma unroll
+            for (int r = 0; r < kPack; ++r) {  // a record's weights stand in its own columns
+              pb[r][nt][0] = kPack == 2 ? w0 & own[r] : w0;
+              pb[r][nt][1] = kPack == 2 ? w1 & own[r] : w1;
+            }
           }
 #pragma unroll
           for (int j = n2 * (W / NG); j < (n2 + 1) * (W / NG); ++j) {
-            // two codes at a time: even rows of O^T get low + 16 high, odd rows 16 high
-            const uint32_t a = v0[j] & 0x00ff00ffu, b = v1[j] & 0x00ff00ffu;
-            const uint32_t a8 = __byte_perm(v0[j], 0, 0x4341), b8 = __byte_perm(v1[j], 0, 0x4341);
+            float d[kNT][4], e[kNT][4];
 #pragma unroll
-            for (int nt = 0; nt < kNT; ++nt) {
-              float d[4], e[4];
-              mma_f16_16816_first(d, a, a8, b, b8, pb[nt][0], pb[nt][1]);
-              mma_f16_16816_first(e, a & 0x00f000f0u, a8 & 0x00f000f0u, b & 0x00f000f0u, b8 & 0x00f000f0u, pb[nt][0],
-                                  pb[nt][1]);
+            for (int r = 0; r < kPack; ++r) {
+              // two codes at a time: even rows of O^T get low + 16 high, odd rows 16 high
+              const uint32_t a = v0[r][j] & 0x00ff00ffu, b = v1[r][j] & 0x00ff00ffu;
+              const uint32_t a8 = __byte_perm(v0[r][j], 0, 0x4341), b8 = __byte_perm(v1[r][j], 0, 0x4341);
+              const uint32_t ah = a & 0x00f000f0u, bh16 = b & 0x00f000f0u, a8h = a8 & 0x00f000f0u, b8h = b8 & 0x00f000f0u;
 #pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                acc[nt][2 * j][c] = add2(acc[nt][2 * j][c], f2(d[2 * c], d[2 * c + 1]));
-                acc[nt][2 * j + 1][c] = add2(acc[nt][2 * j + 1][c], f2(e[2 * c], e[2 * c + 1]));
+              for (int nt = 0; nt < kNT; ++nt) {
+                if (r == 0) {
+                  mma_f16_16816_first(d[nt], a, a8, b, b8, pb[r][nt][0], pb[r][nt][1]);
+                  mma_f16_16816_first(e[nt], ah, a8h, bh16, b8h, pb[r][nt][0], pb[r][nt][1]);
+                } else {
+                  mma_f16_16816(d[nt], a, a8, b, b8, pb[r][nt][0], pb[r][nt][1]);
+                  mma_f16_16816(e[nt], ah, a8h, bh16, b8h, pb[r][nt][0], pb[r][nt][1]);
+                }
               }
             }
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                acc[nt][2 * j][c] = add2(acc[nt][2 * j][c], f2(d[nt][2 * c], d[nt][2 * c + 1]));
+                acc[nt][2 * j + 1][c] = add2(acc[nt][2 * j + 1][c], f2(e[nt][2 * c], e[nt][2 * c + 1]));
+              }
           }
         }
       }
@@ -666,7 +700,8 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
     if (mine > whole_pairs) {
       const uint32_t now = arrived();
       const int u = rs + 2 * (pairs - 1);
-      const int nb = min(kNB, re - u), left = head_len(p, bh) - (u - pre[bh]) * 16;
+      const int nb = min(kNB, re - u);
+      const int left = min(head_len(p, bh) - (u - pre[bh]) * 16, 16 * nb);  // tokens of these records that count
       scores(now, Whole<false>(), nb, left, x, top);
       settle(x, top);
       weigh(now, Whole<false>(), nb, left, x);
@@ -675,6 +710,31 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
     }
 
     // ---- this warp's state of the head into shared memory ----
+    if constexpr (kPack == 2) {  // the two records' columns of a head (lanes t4 and t4 ^ 2) into one
+      float f[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float m = fmaxf(mx[0][c], __shfl_xor_sync(0xffffffff, mx[0][c], 2));
+        f[c] = factor(mx[0][c], m);
+        mx[0][c] = m;
+        l[0][c] *= f[c];
+        l[0][c] += __shfl_xor_sync(0xffffffff, l[0][c], 2);
+#pragma unroll
+        for (int n2 = 0; n2 < NG; ++n2) {
+          um[0][n2][c] *= f[c];
+          um[0][n2][c] += __shfl_xor_sync(0xffffffff, um[0][n2][c], 2);
+        }
+      }
+      const uint64_t both = f2(f[0], f[1]);
+#pragma unroll
+      for (int m = 0; m < 2 * W; ++m)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint64_t v = mul2(acc[0][m][c], both);
+          acc[0][m][c] = add2(v, f2(__shfl_xor_sync(0xffffffff, f2_get(v, 0), 2),
+                                    __shfl_xor_sync(0xffffffff, f2_get(v, 1), 2)));
+        }
+    }
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
@@ -829,7 +889,7 @@ struct DecodeLaunch {
   void* ws;
   cudaStream_t stream;
   int sms, status;
-  template <int D, int NG, int kNT>
+  template <int D, int NG, int kNT, int kPack>
   void launch() {
     using C = Cfg<kNT>;
     const size_t slot = size_t(C::kWarps) * kNB * Kv4<D, NG>::kRec;  // one more slot for every warp
@@ -847,7 +907,7 @@ struct DecodeLaunch {
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 64 || !attr_set[dev]) {
-      if (cudaFuncSetAttribute(kv4_decode_kernel<D, NG, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      if (cudaFuncSetAttribute(kv4_decode_kernel<D, NG, kNT, kPack>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                227 * 1024) != cudaSuccess) {
         status = WGKV_ECUDA;
         return;
@@ -864,12 +924,13 @@ struct DecodeLaunch {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    status = cudaLaunchKernelEx(&cfg, kv4_decode_kernel<D, NG, kNT>, p) == cudaSuccess ? WGKV_OK : WGKV_ECUDA;
+    status = cudaLaunchKernelEx(&cfg, kv4_decode_kernel<D, NG, kNT, kPack>, p) == cudaSuccess ? WGKV_OK : WGKV_ECUDA;
   }
   template <int D, int NG>
   void run() {
-    if (p.G <= 8) launch<D, NG, 1>();
-    else launch<D, NG, 2>();
+    if (p.G <= 4) launch<D, NG, 1, 2>();
+    else if (p.G <= 8) launch<D, NG, 1, 1>();
+    else launch<D, NG, 2, 1>();
   }
 };
 
