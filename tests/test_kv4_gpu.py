@@ -260,6 +260,31 @@ def test_decode_split_over_the_length(wgkv, D, group, Hq, Hk, B, longest):
     within(got, *K4.decode(q, hk, hv, lens, D ** -0.5))
 
 
+@pytest.mark.parametrize("D,group,G", [(128, 64, 4), (64, 32, 8), (128, 128, 12)])
+def test_decode_long_flat_softmax_keeps_its_precision(wgkv, D, group, G):
+    """Millions of records over V's that cancel: the result is hundreds of times smaller than the sums of
+    codes behind it, so rounding that is biased (an accumulation that truncates) shows.
+
+    The bound, in the 2-norm: the output's rounding to bf16 is uniform over half steps of at most 2^-8,
+    2^-8 / sqrt(3) = 2.26e-3; the weights' rounding to fp16, at most 2^-11 each and independent, leaves
+    2^-11 / sqrt(3) times rms(scale * code) / rms(v) = 2.5 for normal V, 7e-4; together 2.4e-3."""
+    rng = np.random.default_rng(D + G)
+    B, Hk, n, T = 16, 4, 54000, 16
+    one = np.array([[n]], np.int32)
+    cache, tbl, hk, hv = filled(wgkv, rng, one, D, group, T,
+                                rows=[K4.bf16(rng.standard_normal((1, 1, n, D))) for _ in range(2)])
+    q = K4.bf16(rng.standard_normal((B, 1, Hk * G, D)) * 0.3)
+    shared = dev_i(tbl).expand(B, Hk, -1)  # every head on the same pages: 64 heads of work, one of memory
+    out = wgkv.paged_decode_kv4(dev(q), cache, dev_i(np.full((B, Hk), n)), shared, D ** -0.5)
+    wgkv.check_errors()
+    k, v = K4.values(*hk[0][0]), K4.values(*hv[0][0])
+    x = q.reshape(-1, D) @ k.T * D ** -0.5
+    p = np.exp(x - x.max(-1, keepdims=True))
+    want = (p @ v / p.sum(-1, keepdims=True)).reshape(q.shape)
+    err = np.linalg.norm(out.double().cpu().numpy() - want) / np.linalg.norm(want)
+    assert err <= 2.4e-3, err
+
+
 @pytest.mark.parametrize("D,group", COMBOS)
 def test_decode_extreme_values(wgkv, D, group):
     """Queries and rows of very different sizes: tokens whose V is tiny but whose weight is 1 next to huge
