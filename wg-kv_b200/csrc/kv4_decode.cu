@@ -45,25 +45,25 @@ constexpr int kLaneHeads = 8;  // heads per lane up to which a warp sums up all 
 constexpr int kMaxBH = 4096;
 constexpr int kMaxG = 16;
 
-// Registers decide: 168 a thread for one tile of 8 query heads (2 CTAs of 6 warps per SM; 8 warps of 128
-// spill and are slower), 255 for two (one CTA of 8 warps).
-template <int kNT>
-struct Cfg {
-  static constexpr int kWarps = kNT == 1 ? 6 : 8;
-  static constexpr int kCtas = kNT == 1 ? 2 : 1;  // per SM
-  static constexpr int kThreads = 32 * kWarps;
-  static constexpr int kMinSegment = kWarps * kNB;  // records a CTA gets at least
-  // A CTA that meets a head's end spends about as long on the merge and the next head's start as on this
-  // many records: segments are cut at the heads' ends where that makes them no longer than this.
-  static constexpr int kAlignSlack = 16;
-};
+// 6 warps of 168 registers in two CTAs per SM.  8 warps of 128 spill (112 us against 97 at 3.5M tokens x
+// heads), 12 warps in one CTA all wait where a head ends (106 us).
+constexpr int kWarps = 6;
+constexpr int kCtas = 2;  // per SM
+constexpr int kThreads = 32 * kWarps;
+constexpr int kMinSegment = kWarps * kNB;  // records a CTA gets at least
+// A CTA that meets a head's end spends about as long on the merge and the next head's start as on this
+// many records: segments are cut at the heads' ends where that makes them no longer than this.
+constexpr int kAlignSlack = 16;
 
 struct Kv4DecodeParams {
   Kv4Pages c;
   const uint16_t* q;
   uint16_t* out;
   const int32_t* seqlens;
-  int BH, G, slots;
+  int group;      // query heads per KV head
+  int halves;     // 1 where a KV head's query heads are worked on as two heads of up to 8 (else 0)
+  int BH, G;      // heads worked on, query heads of each (one fewer in a second half, if group is odd)
+  int slots;
   float scale_log2;
   float* part;    // partial results: (BH + CTAs) x G x (D + 4)
   int* counters;  // per head
@@ -177,24 +177,26 @@ WGKV_DEV void store_out(uint16_t* out, const float4& A, float L) {
   *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(A.x / L, A.y / L), pack_bf16x2(A.z / L, A.w / L));
 }
 
-size_t fixed_smem(int BH, int G, int D, int warps) {
-  return 128 + size_t(warps) * G * (D + 4) * 4 + warps * 32 * 32 + warps * kMaxSlots * 8 +
-         size_t(2 * BH + 34 * warps) * 4 + 64;
+size_t fixed_smem(int BH, int G, int D) {
+  return 128 + size_t(kWarps) * G * (D + 4) * 4 + kThreads * 32 + kWarps * kMaxSlots * 8 +
+         size_t(2 * BH + kThreads + 2 * kWarps) * 4 + 64;
 }
 
 // Tokens of head bh that count: not below 0, not past the table.
 WGKV_DEV int head_len(const Kv4DecodeParams& p, int bh) {
-  return min(max(__ldg(p.seqlens + bh), 0), p.c.width * p.c.page);
+  return min(max(__ldg(p.seqlens + (bh >> p.halves)), 0), p.c.width * p.c.page);
 }
 
-// kNT: 8-head tiles of query heads (G <= 8: 1, G <= 16: 2).  kPack: records whose scores share the 8
-// columns of a tile (G <= 4: 2).
-template <int D, int NG, int kNT, int kPack>
-__global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decode_kernel(Kv4DecodeParams p) {
+// The first query head (row of q and out) of head bh.
+WGKV_DEV size_t query_row(const Kv4DecodeParams& p, int bh) {
+  return size_t(bh >> p.halves) * p.group + (bh & p.halves) * p.G;
+}
+
+// kPack: records whose scores share the 8 columns of a tile: 2 for up to 4 query heads, else 1.
+template <int D, int NG, int kPack>
+__global__ void __launch_bounds__(kThreads, kCtas) kv4_decode_kernel(Kv4DecodeParams p) {
   using F = Kv4<D, NG>;
-  constexpr int kWarps = Cfg<kNT>::kWarps, kThreads = Cfg<kNT>::kThreads;
-  constexpr int kSets = kNB / kPack;        // sets of columns a pair of records fills
-  static_assert(kPack == 1 || (kPack == 2 && kNT == 1), "two records share one tile of columns");
+  constexpr int kSets = kNB / kPack;  // sets of columns that a pair of records fills
   constexpr int W = D / 32;
   constexpr int kMR = merge_row<D>();
   extern __shared__ uint8_t smem_raw[];
@@ -234,10 +236,10 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
 #pragma unroll
     for (int k = 0; k < kLaneHeads; ++k) sum += n[k];
     const int U = __reduce_add_sync(0xffffffff, sum);
-    seg = max(Cfg<kNT>::kMinSegment, (U + int(gridDim.x) - 1) / int(gridDim.x));
+    seg = max(kMinSegment, (U + int(gridDim.x) - 1) / int(gridDim.x));
     // segments that end with the heads, if slightly longer ones are then few enough
-    if (U / (seg + Cfg<kNT>::kAlignSlack) + BH / 2 <= int(gridDim.x)) {
-      for (int more = 0; more <= Cfg<kNT>::kAlignSlack; more += more ? more : 2) {
+    if (U / (seg + kAlignSlack) + BH / 2 <= int(gridDim.x)) {
+      for (int more = 0; more <= kAlignSlack; more += more ? more : 2) {
         const int longer = seg + more;
         int ctas = 0;
 #pragma unroll
@@ -288,7 +290,7 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
       run += (head_len(p, i) + 15) >> 4;
       fin[i] = run;
     }
-    seg = max(Cfg<kNT>::kMinSegment, (U + int(gridDim.x) - 1) / int(gridDim.x));
+    seg = max(kMinSegment, (U + int(gridDim.x) - 1) / int(gridDim.x));
     u0 = min(U, int(blockIdx.x) * seg);
     u1 = min(U, u0 + seg);
     __syncthreads();
@@ -300,10 +302,11 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
       else hi = mid;
     }
   }
+  auto rows_of = [&](int bh) { return min(G, p.group - (bh & p.halves) * G); };  // query heads of head bh
   for (int bh = blockIdx.x; bh < BH; bh += gridDim.x) {  // heads that hold nothing, lengths past the table
     if (fin[bh] == pre[bh])
-      for (int e = tid; e < G * D; e += kThreads) p.out[size_t(bh) * G * D + e] = 0;
-    if (tid == 0 && __ldg(p.seqlens + bh) > p.c.width * p.c.page) set_error(p.c.err, WGKV_ERR_HEAD_CAPACITY);
+      for (int e = tid; e < rows_of(bh) * D; e += kThreads) p.out[query_row(p, bh) * D + e] = 0;
+    if (tid == 0 && __ldg(p.seqlens + (bh >> p.halves)) > p.c.width * p.c.page) set_error(p.c.err, WGKV_ERR_HEAD_CAPACITY);
   }
   if (u0 >= u1) return;
 
@@ -312,17 +315,13 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
   // kPack = 2: columns 0-3 are the heads for the first record of a pair, columns 4-7 for the second
   const int half = kPack == 2 ? t4 >> 1 : 0;
   const uint32_t own[2] = {g < 4 ? 0xffffffffu : 0u, g < 4 ? 0u : 0xffffffffu};
-  uint4 raw_q[kNT][W];
+  uint4 raw_q[W];
   auto load_q = [&](int bh) {
+    const int head = kPack == 2 ? g & 3 : g;
+    const uint16_t* src = p.q + (query_row(p, bh) + head) * D + 8 * t4;
 #pragma unroll
-    for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const int head = kPack == 2 ? g & 3 : nt * 8 + g;
-        raw_q[nt][j] = make_uint4(0, 0, 0, 0);
-        if (head < G)
-          raw_q[nt][j] = __ldg(reinterpret_cast<const uint4*>(p.q + (size_t(bh) * G + head) * D + 32 * j + 8 * t4));
-      }
+    for (int j = 0; j < W; ++j)
+      raw_q[j] = head < rows_of(bh) ? __ldg(reinterpret_cast<const uint4*>(src + 32 * j)) : make_uint4(0, 0, 0, 0);
   };
   while (fin[lo] <= u0) ++lo;  // past heads that hold nothing
   load_q(lo);
@@ -344,7 +343,7 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
         const int u = first + 2 * (warp + kWarps * o) + (lane & 1);
         if (u < last) {
           const uint32_t ul = u - pre[h], pg = upp == 1 ? ul : ul / uint32_t(upp);
-          f_page = __ldg(p.c.table + int64_t(h) * p.c.table_stride + pg);
+          f_page = __ldg(p.c.table + int64_t(h >> p.halves) * p.c.table_stride + pg);
           f_rec = ul - pg * upp;
         }
         break;
@@ -396,80 +395,73 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
     if (re <= rs) continue;
 
     // ---- queries: B fragments, power of two, sums over each group ----
-    uint32_t qf[kNT][W][4];       // [word of K][even k-step b0, b1, odd k-step b0, b1]
-    float qs[kNT][NG][2];         // scale_log2 * sum of the group's q, heads 2 t4 and 2 t4 + 1 of the tile
-    float alpha[kNT][2];          // what a product of codes and fragments is times x's scale
+    uint32_t qf[W][4];       // [word of K][even k-step b0, b1, odd k-step b0, b1]
+    float qs[NG][2];         // scale_log2 * sum of the group's q, heads 2 t4 and 2 t4 + 1 of the tile
+    float alpha[2];          // what a product of codes and fragments is times x's scale
+    float qv[W][8];
+    float big = 0.f;
 #pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
-      float qv[W][8];
-      float big = 0.f;
+    for (int j = 0; j < W; ++j) {
+      unpack8(raw_q[j], qv[j]);
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        unpack8(raw_q[nt][j], qv[j]);
+      for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(qv[j][e]));
+    }
+    big = fmaxf(big, __shfl_xor_sync(0xffffffff, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffff, big, 2));
+    // 2^(14 - exponent(big)), it and its inverse times 2^24 kept normal numbers: smaller exponents count
+    // as -112; a query of 2^118 or more overflows (to NaN)
+    const int ex = min(max(int(__float_as_uint(big) >> 23) - 127, -112), 117);
+    const float up = __uint_as_float(uint32_t(14 - ex + 127) << 23);
+    float sum[NG];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(qv[j][e]));
+    for (int n = 0; n < NG; ++n) sum[n] = 0.f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        sum[j * NG / W] += qv[j][e];
+        qv[j][e] *= up;
       }
-      big = fmaxf(big, __shfl_xor_sync(0xffffffff, big, 1));
-      big = fmaxf(big, __shfl_xor_sync(0xffffffff, big, 2));
-      // 2^(14 - exponent(big)), it and its inverse times 2^24 kept normal numbers: smaller exponents count
-      // as -112; a query of 2^118 or more overflows (to NaN)
-      const int ex = min(max(int(__float_as_uint(big) >> 23) - 127, -112), 117);
-      const float up = __uint_as_float(uint32_t(14 - ex + 127) << 23);
-      float sum[NG];
+      qf[j][0] = pack_f16x2(qv[j][0], qv[j][4]);
+      qf[j][1] = pack_f16x2(qv[j][2], qv[j][6]);
+      qf[j][2] = pack_f16x2(qv[j][1] * 0.0625f, qv[j][5] * 0.0625f);
+      qf[j][3] = pack_f16x2(qv[j][3] * 0.0625f, qv[j][7] * 0.0625f);
+    }
+    // 2^24 (the codes') / up (the queries'), as 2^(24 - 14 + ex): the lanes of heads 2 t4 and 2 t4 + 1 have it
+    const float a = p.scale_log2 * __uint_as_float(uint32_t(10 + ex + 127) << 23);
 #pragma unroll
-      for (int n = 0; n < NG; ++n) sum[n] = 0.f;
+    for (int c = 0; c < 2; ++c) alpha[c] = __shfl_sync(0xffffffff, a, (2 * t4 + c) * 4);
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
+    for (int n = 0; n < NG; ++n) {
+      sum[n] += __shfl_xor_sync(0xffffffff, sum[n], 1);
+      sum[n] += __shfl_xor_sync(0xffffffff, sum[n], 2);
+      sum[n] *= p.scale_log2;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          sum[j * NG / W] += qv[j][e];
-          qv[j][e] *= up;
-        }
-        qf[nt][j][0] = pack_f16x2(qv[j][0], qv[j][4]);
-        qf[nt][j][1] = pack_f16x2(qv[j][2], qv[j][6]);
-        qf[nt][j][2] = pack_f16x2(qv[j][1] * 0.0625f, qv[j][5] * 0.0625f);
-        qf[nt][j][3] = pack_f16x2(qv[j][3] * 0.0625f, qv[j][7] * 0.0625f);
-      }
-      // 2^24 (the codes') / up (the queries'), as 2^(24 - 14 + ex): the lanes of heads 2 t4 and 2 t4 + 1 have it
-      const float a = p.scale_log2 * __uint_as_float(uint32_t(10 + ex + 127) << 23);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) alpha[nt][c] = __shfl_sync(0xffffffff, a, (2 * t4 + c) * 4);
-#pragma unroll
-      for (int n = 0; n < NG; ++n) {
-        sum[n] += __shfl_xor_sync(0xffffffff, sum[n], 1);
-        sum[n] += __shfl_xor_sync(0xffffffff, sum[n], 2);
-        sum[n] *= p.scale_log2;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) qs[nt][n][c] = __shfl_sync(0xffffffff, sum[n], (2 * t4 + c) * 4);
-      }
+      for (int c = 0; c < 2; ++c) qs[n][c] = __shfl_sync(0xffffffff, sum[n], (2 * t4 + c) * 4);
     }
 
-    uint64_t acc[kNT][2 * W][2];  // O^T: m-tile, row g and g + 8, heads 2 t4 and 2 t4 + 1 as an fp32 pair
-    float um[kNT][NG][2];         // sum of p m_v over this lane's tokens
-    float mx[kNT][2], l[kNT][2];
+    uint64_t acc[2 * W][2];  // O^T: m-tile, row g and g + 8, heads 2 t4 and 2 t4 + 1 as an fp32 pair
+    float um[NG][2];         // sum of p m_v over this lane's tokens
+    float mx[2], l[2];
 #pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
+    for (int m = 0; m < 2 * W; ++m) acc[m][0] = acc[m][1] = 0;
 #pragma unroll
-      for (int m = 0; m < 2 * W; ++m) acc[nt][m][0] = acc[nt][m][1] = 0;
+    for (int c = 0; c < 2; ++c) {
+      mx[c] = 0.f;
+      l[c] = 0.f;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        mx[nt][c] = 0.f;
-        l[nt][c] = 0.f;
-#pragma unroll
-        for (int n = 0; n < NG; ++n) um[nt][n][c] = 0.f;
-      }
+      for (int n = 0; n < NG; ++n) um[n][c] = 0.f;
     }
 
     bool first = true;  // no reference yet
     struct Scores {
-      float v[kSets][kNT][4];
+      float v[kSets][4];
     };
     // Scores of a pair of records relative to the reference, and a bound of their weights.  kAll: both are
     // there and every token counts, so that nothing branches.
-    auto scores = [&](uint32_t recs, auto all, int nb, int left, Scores& x, float (&top)[kNT][2]) {
+    auto scores = [&](uint32_t recs, auto all, int nb, int left, Scores& x, float (&top)[2]) {
       constexpr bool kAll = decltype(all)::value;
-#pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
+      top[0] = top[1] = -INFINITY;
 #pragma unroll
       for (int i = 0; i < kSets; ++i) {
         if (!kAll && i >= nb) continue;
@@ -483,41 +475,35 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
         const uint32_t rec = recs + mine * F::kRec;
         lds_words<NG>(kp0, rec + F::kKP + g * 4 * NG);
         lds_words<NG>(kp1, rec + F::kKP + (g + 8) * 4 * NG);
-        float t[kNT][4], o[kNT][4];
+        float t[4], o[4];
 #pragma unroll
         for (int n2 = 0; n2 < NG; ++n2) {
-          float d[kPack][kNT][4];
+          float d[kPack][4];
 #pragma unroll
           for (int j = n2 * (W / NG); j < (n2 + 1) * (W / NG); ++j) {
 #pragma unroll
             for (int r = 0; r < kPack; ++r) {
               const uint32_t a = k0[r][j], b = k1[r][j], a8 = a >> 8, b8 = b >> 8;
-#pragma unroll
-              for (int nt = 0; nt < kNT; ++nt) {
-                if (j == n2 * (W / NG))
-                  mma_f16_16816_first(d[r][nt], a & 0x000f000fu, b & 0x000f000fu, a8 & 0x000f000fu, b8 & 0x000f000fu,
-                                      qf[nt][j][0], qf[nt][j][1]);
-                else
-                  mma_f16_16816(d[r][nt], a & 0x000f000fu, b & 0x000f000fu, a8 & 0x000f000fu, b8 & 0x000f000fu,
-                                qf[nt][j][0], qf[nt][j][1]);
-                mma_f16_16816(d[r][nt], a & 0x00f000f0u, b & 0x00f000f0u, a8 & 0x00f000f0u, b8 & 0x00f000f0u,
-                              qf[nt][j][2], qf[nt][j][3]);
-              }
+              if (j == n2 * (W / NG))
+                mma_f16_16816_first(d[r], a & 0x000f000fu, b & 0x000f000fu, a8 & 0x000f000fu, b8 & 0x000f000fu,
+                                    qf[j][0], qf[j][1]);
+              else
+                mma_f16_16816(d[r], a & 0x000f000fu, b & 0x000f000fu, a8 & 0x000f000fu, b8 & 0x000f000fu, qf[j][0],
+                              qf[j][1]);
+              mma_f16_16816(d[r], a & 0x00f000f0u, b & 0x00f000f0u, a8 & 0x00f000f0u, b8 & 0x00f000f0u, qf[j][2],
+                            qf[j][3]);
             }
           }
           const float s0 = __uint_as_float(kp0[n2] & 0xffff0000u), m0 = __uint_as_float(kp0[n2] << 16);
           const float s1 = __uint_as_float(kp1[n2] & 0xffff0000u), m1 = __uint_as_float(kp1[n2] << 16);
 #pragma unroll
-          for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const float d0 = kPack == 2 && half ? d[kPack - 1][nt][c] : d[0][nt][c];
-              const float d1 = kPack == 2 && half ? d[kPack - 1][nt][2 + c] : d[0][nt][2 + c];
-              t[nt][c] = n2 ? fmaf(s0, d0, t[nt][c]) : s0 * d0;
-              t[nt][2 + c] = n2 ? fmaf(s1, d1, t[nt][2 + c]) : s1 * d1;
-              o[nt][c] = fmaf(m0, qs[nt][n2][c], n2 ? o[nt][c] : -mx[nt][c]);
-              o[nt][2 + c] = fmaf(m1, qs[nt][n2][c], n2 ? o[nt][2 + c] : -mx[nt][c]);
-            }
+          for (int c = 0; c < 2; ++c) {
+            const float d0 = kPack == 2 && half ? d[kPack - 1][c] : d[0][c];
+            const float d1 = kPack == 2 && half ? d[kPack - 1][2 + c] : d[0][2 + c];
+            t[c] = n2 ? fmaf(s0, d0, t[c]) : s0 * d0;
+            t[2 + c] = n2 ? fmaf(s1, d1, t[2 + c]) : s1 * d1;
+            o[c] = fmaf(m0, qs[n2][c], n2 ? o[c] : -mx[c]);
+            o[2 + c] = fmaf(m1, qs[n2][c], n2 ? o[2 + c] : -mx[c]);
           }
         }
         // 2^23 + biased exponent of the largest scale of each token's V row (at least -40): added to x it
@@ -534,53 +520,44 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
         const float e0 = __uint_as_float(0x4b000000u | v0 >> 23), e1 = __uint_as_float(0x4b000000u | v1 >> 23);
         const int valid = left - 16 * mine;
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const float y = fmaf(alpha[nt][c & 1], t[nt][c], o[nt][c]);
-            x.v[i][nt][c] = kAll || g + 8 * (c >> 1) < valid ? y : -INFINITY;
-          }
-          top[nt][0] = fmaxf(top[nt][0], fmaxf(x.v[i][nt][0] + e0, x.v[i][nt][2] + e1));
-          top[nt][1] = fmaxf(top[nt][1], fmaxf(x.v[i][nt][1] + e0, x.v[i][nt][3] + e1));
+        for (int c = 0; c < 4; ++c) {
+          const float y = fmaf(alpha[c & 1], t[c], o[c]);
+          x.v[i][c] = kAll || g + 8 * (c >> 1) < valid ? y : -INFINITY;
         }
+        top[0] = fmaxf(top[0], fmaxf(x.v[i][0] + e0, x.v[i][2] + e1));
+        top[1] = fmaxf(top[1], fmaxf(x.v[i][1] + e0, x.v[i][3] + e1));
       }
     };
     // Moves the reference where a weight would outgrow it: most pairs only learn that none does.
-    auto settle = [&](Scores& x, const float (&top)[kNT][2]) {
-      bool move = first;
+    auto settle = [&](Scores& x, const float (&top)[2]) {
+      if (__any_sync(0xffffffff, first || fmaxf(top[0], top[1]) > 8388608.f + 127.f + 8.f)) {
+        float fac[2];
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) move |= fmaxf(top[nt][0], top[nt][1]) > 8388608.f + 127.f + 8.f;
-      if (__any_sync(0xffffffff, move)) {
+        for (int c = 0; c < 2; ++c) {
+          float m = top[c];
+          m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 4));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 8));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 16));
+          m -= 8388608.f + 127.f;
+          // up by `by`, where that is positive; the first time to where it belongs (a floor keeps it finite)
+          const float by = fmaxf(m, first ? -1e30f : 0.f);
+          const float f = first ? 0.f : exp2_approx(-by);
+          mx[c] += by;
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) {
-          float fac[2];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float m = top[nt][c];
-            m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 4));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 8));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 16));
-            m -= 8388608.f + 127.f;
-            // up by `by`, where that is positive; the first time to where it belongs (a floor keeps it finite)
-            const float by = fmaxf(m, first ? -1e30f : 0.f);
-            const float f = first ? 0.f : exp2_approx(-by);
-            mx[nt][c] += by;
-#pragma unroll
-            for (int i = 0; i < kSets; ++i) {
-              x.v[i][nt][c] -= by;
-              x.v[i][nt][2 + c] -= by;
-            }
-            l[nt][c] *= f;
-#pragma unroll
-            for (int n2 = 0; n2 < NG; ++n2) um[nt][n2][c] *= f;
-            fac[c] = f;
+          for (int i = 0; i < kSets; ++i) {
+            x.v[i][c] -= by;
+            x.v[i][2 + c] -= by;
           }
-          const uint64_t both = f2(fac[0], fac[1]);
+          l[c] *= f;
 #pragma unroll
-          for (int m2 = 0; m2 < 2 * W; ++m2) {
-            acc[nt][m2][0] = mul2(acc[nt][m2][0], both);
-            acc[nt][m2][1] = mul2(acc[nt][m2][1], both);
-          }
+          for (int n2 = 0; n2 < NG; ++n2) um[n2][c] *= f;
+          fac[c] = f;
+        }
+        const uint64_t both = f2(fac[0], fac[1]);
+#pragma unroll
+        for (int m2 = 0; m2 < 2 * W; ++m2) {
+          acc[m2][0] = mul2(acc[m2][0], both);
+          acc[m2][1] = mul2(acc[m2][1], both);
         }
         first = false;
       }
@@ -602,14 +579,11 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
           lds_words<W>(v0[r], recs + (i + r) * F::kRec + F::kV + lane * (D / 8));
           lds_words<W>(v1[r], recs + (i + r) * F::kRec + F::kV + 4 * D + lane * (D / 8));
         }
-        float pr[kNT][4];
+        float pr[4];
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) pr[nt][c] = exp2_approx(x.v[i][nt][c]);
-          l[nt][0] += pr[nt][0] + pr[nt][2];
-          l[nt][1] += pr[nt][1] + pr[nt][3];
-        }
+        for (int c = 0; c < 4; ++c) pr[c] = exp2_approx(x.v[i][c]);
+        l[0] += pr[0] + pr[2];
+        l[1] += pr[1] + pr[3];
 #pragma unroll
         for (int n2 = 0; n2 < NG; ++n2) {
           if (!kAll) {  // places behind the length may hold anything
@@ -618,46 +592,38 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
           }
           const float s0 = __uint_as_float(vp0[n2] & 0xffff0000u), m0 = __uint_as_float(vp0[n2] << 16);
           const float s1 = __uint_as_float(vp1[n2] & 0xffff0000u), m1 = __uint_as_float(vp1[n2] << 16);
-          uint32_t pb[kPack][kNT][2];
+          uint32_t pb[kPack][2];
+          um[n2][0] = fmaf(pr[0], m0, fmaf(pr[2], m1, um[n2][0]));
+          um[n2][1] = fmaf(pr[1], m0, fmaf(pr[3], m1, um[n2][1]));
+          const uint32_t w0 = movmatrix_trans(pack_f16x2(pr[0] * s0, pr[1] * s0));
+          const uint32_t w1 = movmatrix_trans(pack_f16x2(pr[2] * s1, pr[3] * s1));
 #pragma unroll
-          for (int nt = 0; nt < kNT; ++nt) {
-            um[nt][n2][0] = fmaf(pr[nt][0], m0, fmaf(pr[nt][2], m1, um[nt][n2][0]));
-            um[nt][n2][1] = fmaf(pr[nt][1], m0, fmaf(pr[nt][3], m1, um[nt][n2][1]));
-            const uint32_t w0 = movmatrix_trans(pack_f16x2(pr[nt][0] * s0, pr[nt][1] * s0));
-            const uint32_t w1 = movmatrix_trans(pack_f16x2(pr[nt][2] * s1, pr[nt][3] * s1));
-#pragma unroll
-            for (int r = 0; r < kPack; ++r) {  // a record's weights stand in its own columns
-              pb[r][nt][0] = kPack == 2 ? w0 & own[r] : w0;
-              pb[r][nt][1] = kPack == 2 ? w1 & own[r] : w1;
-            }
+          for (int r = 0; r < kPack; ++r) {  // a record's weights stand in its own columns
+            pb[r][0] = kPack == 2 ? w0 & own[r] : w0;
+            pb[r][1] = kPack == 2 ? w1 & own[r] : w1;
           }
 #pragma unroll
           for (int j = n2 * (W / NG); j < (n2 + 1) * (W / NG); ++j) {
-            float d[kNT][4], e[kNT][4];
+            float d[4], e[4];
 #pragma unroll
             for (int r = 0; r < kPack; ++r) {
               // two codes at a time: even rows of O^T get low + 16 high, odd rows 16 high
               const uint32_t a = v0[r][j] & 0x00ff00ffu, b = v1[r][j] & 0x00ff00ffu;
               const uint32_t a8 = __byte_perm(v0[r][j], 0, 0x4341), b8 = __byte_perm(v1[r][j], 0, 0x4341);
               const uint32_t ah = a & 0x00f000f0u, bh16 = b & 0x00f000f0u, a8h = a8 & 0x00f000f0u, b8h = b8 & 0x00f000f0u;
-#pragma unroll
-              for (int nt = 0; nt < kNT; ++nt) {
-                if (r == 0) {
-                  mma_f16_16816_first(d[nt], a, a8, b, b8, pb[r][nt][0], pb[r][nt][1]);
-                  mma_f16_16816_first(e[nt], ah, a8h, bh16, b8h, pb[r][nt][0], pb[r][nt][1]);
-                } else {
-                  mma_f16_16816(d[nt], a, a8, b, b8, pb[r][nt][0], pb[r][nt][1]);
-                  mma_f16_16816(e[nt], ah, a8h, bh16, b8h, pb[r][nt][0], pb[r][nt][1]);
-                }
+              if (r == 0) {
+                mma_f16_16816_first(d, a, a8, b, b8, pb[r][0], pb[r][1]);
+                mma_f16_16816_first(e, ah, a8h, bh16, b8h, pb[r][0], pb[r][1]);
+              } else {
+                mma_f16_16816(d, a, a8, b, b8, pb[r][0], pb[r][1]);
+                mma_f16_16816(e, ah, a8h, bh16, b8h, pb[r][0], pb[r][1]);
               }
             }
 #pragma unroll
-            for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                acc[nt][2 * j][c] = add2(acc[nt][2 * j][c], f2(d[nt][2 * c], d[nt][2 * c + 1]));
-                acc[nt][2 * j + 1][c] = add2(acc[nt][2 * j + 1][c], f2(e[nt][2 * c], e[nt][2 * c + 1]));
-              }
+            for (int c = 0; c < 2; ++c) {
+              acc[2 * j][c] = add2(acc[2 * j][c], f2(d[2 * c], d[2 * c + 1]));
+              acc[2 * j + 1][c] = add2(acc[2 * j + 1][c], f2(e[2 * c], e[2 * c + 1]));
+            }
           }
         }
       }
@@ -677,7 +643,7 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
       return recs;
     };
     Scores x;
-    float top[kNT][2];
+    float top[2];
     if (whole_pairs > 0) {
       uint32_t now = arrived();
       scores(now, Whole<true>(), kNB, 0, x, top);
@@ -714,15 +680,15 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
       float f[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const float m = fmaxf(mx[0][c], __shfl_xor_sync(0xffffffff, mx[0][c], 2));
-        f[c] = factor(mx[0][c], m);
-        mx[0][c] = m;
-        l[0][c] *= f[c];
-        l[0][c] += __shfl_xor_sync(0xffffffff, l[0][c], 2);
+        const float m = fmaxf(mx[c], __shfl_xor_sync(0xffffffff, mx[c], 2));
+        f[c] = factor(mx[c], m);
+        mx[c] = m;
+        l[c] *= f[c];
+        l[c] += __shfl_xor_sync(0xffffffff, l[c], 2);
 #pragma unroll
         for (int n2 = 0; n2 < NG; ++n2) {
-          um[0][n2][c] *= f[c];
-          um[0][n2][c] += __shfl_xor_sync(0xffffffff, um[0][n2][c], 2);
+          um[n2][c] *= f[c];
+          um[n2][c] += __shfl_xor_sync(0xffffffff, um[n2][c], 2);
         }
       }
       const uint64_t both = f2(f[0], f[1]);
@@ -730,42 +696,41 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
       for (int m = 0; m < 2 * W; ++m)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const uint64_t v = mul2(acc[0][m][c], both);
-          acc[0][m][c] = add2(v, f2(__shfl_xor_sync(0xffffffff, f2_get(v, 0), 2),
+          const uint64_t v = mul2(acc[m][c], both);
+          acc[m][c] = add2(v, f2(__shfl_xor_sync(0xffffffff, f2_get(v, 0), 2),
                                     __shfl_xor_sync(0xffffffff, f2_get(v, 1), 2)));
         }
     }
+    const int rows = rows_of(bh);
 #pragma unroll
-    for (int nt = 0; nt < kNT; ++nt)
+    for (int c = 0; c < 2; ++c) {
+      const int head = 2 * t4 + c;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int head = nt * 8 + 2 * t4 + c;
+      for (int o = 4; o < 32; o <<= 1) {
+        l[c] += __shfl_xor_sync(0xffffffff, l[c], o);
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-          l[nt][c] += __shfl_xor_sync(0xffffffff, l[nt][c], o);
+        for (int n2 = 0; n2 < NG; ++n2) um[n2][c] += __shfl_xor_sync(0xffffffff, um[n2][c], o);
+      }
+      if (head < rows) {
+        float* row = merge + (warp * G + head) * kMR;
 #pragma unroll
-          for (int n2 = 0; n2 < NG; ++n2) um[nt][n2][c] += __shfl_xor_sync(0xffffffff, um[nt][n2][c], o);
+        for (int j = 0; j < W; ++j) {
+          const float m = um[j * NG / W][c];
+          const float e0 = f2_get(acc[2 * j][0], c), o0 = f2_get(acc[2 * j + 1][0], c);
+          const float e1 = f2_get(acc[2 * j][1], c), o1 = f2_get(acc[2 * j + 1][1], c);
+          float4 v;
+          v.x = fmaf(e0 - o0, 16777216.f, m);
+          v.y = fmaf(o0, 1048576.f, m);
+          v.z = fmaf(e1 - o1, 16777216.f, m);
+          v.w = fmaf(o1, 1048576.f, m);
+          *reinterpret_cast<float4*>(row + 32 * j + 4 * g) = v;
         }
-        if (head < G) {
-          float* row = merge + (warp * G + head) * kMR;
-#pragma unroll
-          for (int j = 0; j < W; ++j) {
-            const float m = um[nt][j * NG / W][c];
-            const float e0 = f2_get(acc[nt][2 * j][0], c), o0 = f2_get(acc[nt][2 * j + 1][0], c);
-            const float e1 = f2_get(acc[nt][2 * j][1], c), o1 = f2_get(acc[nt][2 * j + 1][1], c);
-            float4 v;
-            v.x = fmaf(e0 - o0, 16777216.f, m);
-            v.y = fmaf(o0, 1048576.f, m);
-            v.z = fmaf(e1 - o1, 16777216.f, m);
-            v.w = fmaf(o1, 1048576.f, m);
-            *reinterpret_cast<float4*>(row + 32 * j + 4 * g) = v;
-          }
-          if (g == 0) {
-            row[D] = first ? -INFINITY : mx[nt][c];
-            row[D + 1] = l[nt][c];
-          }
+        if (g == 0) {
+          row[D] = first ? -INFINITY : mx[c];
+          row[D + 1] = l[c];
         }
       }
+    }
     // the next head's queries on their way
     int after = bh + 1;
     while (after < BH && fin[after] == pre[after]) ++after;
@@ -774,8 +739,9 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
 
     // ---- the warps' states into one: output, or this CTA's partial result ----
     const bool whole = rs == hs && re == he;
+    uint16_t* out = p.out + query_row(p, bh) * D;
     float* mine_at = p.part + size_t(bh + blockIdx.x) * G * kMR;
-    for (int e = tid; e < G * (D / 4); e += kThreads) {
+    for (int e = tid; e < rows * (D / 4); e += kThreads) {
       const int r = e / (D / 4), d = 4 * (e % (D / 4));
       const float* row = merge + r * kMR;
       float M = -INFINITY;
@@ -789,7 +755,7 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
         add_state(A, L, factor(state[D], M), *reinterpret_cast<const float4*>(state + d), state[D + 1]);
       }
       if (whole) {
-        store_out(p.out + (size_t(bh) * G + r) * D + d, A, L);
+        store_out(out + r * D + d, A, L);
       } else {
         *reinterpret_cast<float4*>(mine_at + r * kMR + d) = A;
         if (d == 0) *reinterpret_cast<float2*>(mine_at + r * kMR + D) = make_float2(M, L);
@@ -811,7 +777,7 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
         // in flight at once; lane i of them reads the i-th one's maximum and sum
         constexpr int kLanes = D / 4, kChunk = 16;
         const float* p0 = p.part + size_t(bh + c_first) * G * kMR;
-        const int cols = G * kLanes;
+        const int cols = rows * kLanes;
         const int parts = kThreads / cols > 1 ? kThreads / cols : 1;
         const int sub = lane % kLanes;
         for (int e = tid; e < cols * parts; e += kThreads) {  // whole groups of kLanes lanes come through together
@@ -848,7 +814,7 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
             }
           }
           if (parts == 1) {
-            store_out(p.out + (size_t(bh) * G + r) * D + d, A, L);
+            store_out(out + r * D + d, A, L);
           } else {
             float* j = join + e * 8;
             *reinterpret_cast<float4*>(j) = A;
@@ -866,7 +832,7 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
               const float* j = join + (c * cols + e) * 8;
               add_state(A, L, factor(j[4], M), *reinterpret_cast<const float4*>(j), j[5]);
             }
-            store_out(p.out + (size_t(bh) * G + r) * D + d, A, L);
+            store_out(out + r * D + d, A, L);
           }
         }
       }
@@ -880,8 +846,17 @@ __global__ void __launch_bounds__(Cfg<kNT>::kThreads, Cfg<kNT>::kCtas) kv4_decod
   }
 }
 
-size_t workspace_bytes(int64_t BH, int G, int D, int grid) {
-  return ((size_t(BH) * 4 + 255) & ~size_t(255)) + size_t(BH + grid) * G * (D + 4) * 4 + 256;
+// More than 8 query heads on a KV head are worked on as two heads: the records' codes are copied and
+// unpacked twice (the second time from L2, as a rule), which costs less than two tiles of accumulators in
+// one warp, whose registers leave 8 warps on an SM (26 us against 22 with 16 query heads, 141K tokens).
+int head_halves(int group) { return group > 8 ? 1 : 0; }
+
+size_t counter_bytes(int64_t BH) { return (size_t(BH) * 4 + 255) & ~size_t(255); }
+
+size_t workspace_need(int64_t kv_heads, int group, int D, int sms) {
+  const int halves = head_halves(group), G = (group + halves) >> halves;
+  const int64_t BH = kv_heads << halves;
+  return counter_bytes(BH) + size_t(BH + sms * kCtas) * G * (D + 4) * 4 + 256;
 }
 
 struct DecodeLaunch {
@@ -889,14 +864,13 @@ struct DecodeLaunch {
   void* ws;
   cudaStream_t stream;
   int sms, status;
-  template <int D, int NG, int kNT, int kPack>
+  template <int D, int NG, int kPack>
   void launch() {
-    using C = Cfg<kNT>;
-    const size_t slot = size_t(C::kWarps) * kNB * Kv4<D, NG>::kRec;  // one more slot for every warp
-    const size_t fixed = fixed_smem(p.BH, p.G, D, C::kWarps);
+    const size_t slot = size_t(kWarps) * kNB * Kv4<D, NG>::kRec;  // one more slot for every warp
+    const size_t fixed = fixed_smem(p.BH, p.G, D);
     // As many slots as fit next to another CTA; with many heads or a large group (their prefix sums and
     // merge rows) a CTA has the SM to itself.
-    size_t room = C::kCtas == 2 ? 227 * 1024 / 2 - 1024 : 227 * 1024;
+    size_t room = 227 * 1024 / kCtas - 1024;
     if (fixed + 2 * slot > room) room = 227 * 1024;
     if (fixed + 2 * slot > room) {
       status = WGKV_EINVAL;
@@ -907,7 +881,7 @@ struct DecodeLaunch {
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 64 || !attr_set[dev]) {
-      if (cudaFuncSetAttribute(kv4_decode_kernel<D, NG, kNT, kPack>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      if (cudaFuncSetAttribute(kv4_decode_kernel<D, NG, kPack>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                227 * 1024) != cudaSuccess) {
         status = WGKV_ECUDA;
         return;
@@ -915,8 +889,8 @@ struct DecodeLaunch {
       if (dev < 64) attr_set[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(sms * C::kCtas);
-    cfg.blockDim = dim3(C::kThreads);
+    cfg.gridDim = dim3(sms * kCtas);
+    cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = fixed + p.slots * slot;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -924,16 +898,14 @@ struct DecodeLaunch {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    status = cudaLaunchKernelEx(&cfg, kv4_decode_kernel<D, NG, kNT, kPack>, p) == cudaSuccess ? WGKV_OK : WGKV_ECUDA;
+    status = cudaLaunchKernelEx(&cfg, kv4_decode_kernel<D, NG, kPack>, p) == cudaSuccess ? WGKV_OK : WGKV_ECUDA;
   }
   template <int D, int NG>
   void run() {
-    if (p.G <= 4) launch<D, NG, 1, 2>();
-    else if (p.G <= 8) launch<D, NG, 1, 1>();
-    else launch<D, NG, 2, 1>();
+    if (p.G <= 4) launch<D, NG, 2>();
+    else launch<D, NG, 1>();
   }
 };
-
 
 }  // namespace
 }  // namespace wgkv
@@ -942,8 +914,8 @@ using namespace wgkv;
 
 extern "C" size_t wgkv_paged_decode_kv4_workspace_size(int batch, int num_q_heads, int num_kv_heads, int head_dim) {
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || head_dim <= 0) return 0;
-  const int sms = device_sms(), G = num_q_heads / num_kv_heads;
-  return workspace_bytes(int64_t(batch) * num_kv_heads, G, head_dim, (sms > 0 ? sms : 148) * (G <= 8 ? Cfg<1>::kCtas : Cfg<2>::kCtas));
+  const int sms = device_sms();
+  return workspace_need(int64_t(batch) * num_kv_heads, num_q_heads / num_kv_heads, head_dim, sms > 0 ? sms : 148);
 }
 
 extern "C" int wgkv_paged_decode_kv4(const uint16_t* q, const uint8_t* cache, int64_t num_pages, int page_size,
@@ -957,24 +929,26 @@ extern "C" int wgkv_paged_decode_kv4(const uint16_t* q, const uint8_t* cache, in
       num_q_heads / num_kv_heads > kMaxG || int64_t(batch) * num_kv_heads > kMaxBH)
     return WGKV_EINVAL;
   if (num_pages <= 0 || page_size <= 0 || page_size % 16 || table_width <= 0 || table_stride < table_width ||
-      int64_t(batch) * num_kv_heads * table_width * (page_size / 16) >= (int64_t(1) << 31) ||
+      int64_t(batch) * num_kv_heads * table_width * (page_size / 16) >= (int64_t(1) << 30) ||
       int64_t(table_width) * page_size >= (int64_t(1) << 31) || num_pages * (page_size / 16) >= (int64_t(1) << 31) ||
       (reinterpret_cast<uintptr_t>(cache) & 15) || (reinterpret_cast<uintptr_t>(q) & 15) ||
       (reinterpret_cast<uintptr_t>(out) & 15) || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return WGKV_EINVAL;
   if (workspace_bytes < wgkv_paged_decode_kv4_workspace_size(batch, num_q_heads, num_kv_heads, head_dim))
     return WGKV_ENOSPC;
-  const int BH = batch * num_kv_heads;
+  const int group_heads = num_q_heads / num_kv_heads, halves = head_halves(group_heads);
   DecodeLaunch a = {};
   a.p.c = {const_cast<uint8_t*>(cache), num_pages, page_size, block_table, table_stride, table_width, err};
   a.p.q = q;
   a.p.out = out;
   a.p.seqlens = cache_seqlens;
-  a.p.BH = BH;
-  a.p.G = num_q_heads / num_kv_heads;
+  a.p.group = group_heads;
+  a.p.halves = halves;
+  a.p.BH = (batch * num_kv_heads) << halves;
+  a.p.G = (group_heads + halves) >> halves;
   a.p.scale_log2 = softmax_scale * 1.4426950408889634f;
   a.p.counters = reinterpret_cast<int*>(workspace);
-  a.p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ((size_t(BH) * 4 + 255) & ~size_t(255)));
+  a.p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + counter_bytes(a.p.BH));
   a.stream = as_stream(stream);
   a.sms = device_sms();
   if (a.sms <= 0) return WGKV_ECUDA;

@@ -305,7 +305,7 @@ def paged_decode_kv4(q, cache, cache_seqlens, block_table, softmax_scale, out=No
     need = _scratch.get(heads)
     if need is None:
         need = _remember(_scratch, heads, (int(lib.wgkv_paged_decode_kv4_workspace_size(B, Hq, Hk, D)),
-                                           (B * Hk * 4 + 255) // 256 * 256))
+                                           (B * Hk * 8 + 255) // 256 * 256))
     stream = raw_stream(index)
     ws, ws_bytes = counter_scratch(index, stream, "paged_decode_kv4", *need)
     _call(index, _DECODE,
