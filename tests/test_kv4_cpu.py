@@ -68,7 +68,7 @@ def test_entry_points_refuse_what_is_theirs():
     for bad in (dict(q=None), dict(q=F + 2), dict(sl=None), dict(out=None), dict(out=F + 8), dict(ws=None),
                 dict(Hq=7), dict(Hq=0), dict(Hq=34), dict(B=2049)):
         assert _decode(**bad) == EINVAL, bad
-    # units of 16 tokens are counted in 32 bits over all heads
+    # records of 16 tokens are counted in 32 bits over all heads
     assert _decode(B=1024, Hk=4, Hq=8, width=1 << 20, stride=1 << 20, page=64) == EINVAL
     assert _decode(nbytes=0) == ENOSPC
     assert _append(L=0) == 0 and _read(rows=0) == 0  # nothing to do, nothing launched

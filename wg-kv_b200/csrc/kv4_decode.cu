@@ -187,6 +187,14 @@ WGKV_DEV int head_len(const Kv4DecodeParams& p, int bh) {
   return min(max(__ldg(p.seqlens + (bh >> p.halves)), 0), p.c.width * p.c.page);
 }
 
+// ceil(n / d) for 0 <= n < 2^30, d > 0: a quotient in fp32 is at most one off.
+WGKV_DEV int ceil_div(int n, int d) {
+  n += d - 1;
+  int q = int(__fdividef(float(n), float(d)));
+  const int r = n - q * d;
+  return r < 0 ? q - 1 : r >= d ? q + 1 : q;
+}
+
 // The first query head (row of q and out) of head bh.
 WGKV_DEV size_t query_row(const Kv4DecodeParams& p, int bh) {
   return size_t(bh >> p.halves) * p.group + (bh & p.halves) * p.G;
@@ -227,30 +235,37 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv4_decode_kernel(Kv4DecodePa
     // each warp for itself (all write the same values): no barrier between the launch and the first copy
     const int per = (BH + 31) >> 5;
     int n[kLaneHeads], room[kLaneHeads], sum = 0;
+    bool over = false;
 #pragma unroll
     for (int k = 0; k < kLaneHeads; ++k) {
       const int i = lane * per + k;
-      n[k] = k < per && i < BH ? (head_len(p, i) + 15) >> 4 : 0;
+      const int len = k < per && i < BH ? __ldg(p.seqlens + (i >> p.halves)) : 0;
+      over |= len > p.c.width * p.c.page;
+      n[k] = (min(max(len, 0), p.c.width * p.c.page) + 15) >> 4;
       room[k] = n[k];
     }
+    if (over && blockIdx.x == 0) set_error(p.c.err, WGKV_ERR_HEAD_CAPACITY);
 #pragma unroll
     for (int k = 0; k < kLaneHeads; ++k) sum += n[k];
     const int U = __reduce_add_sync(0xffffffff, sum);
-    seg = max(kMinSegment, (U + int(gridDim.x) - 1) / int(gridDim.x));
+    seg = max(kMinSegment, ceil_div(U, gridDim.x));
     // segments that end with the heads, if slightly longer ones are then few enough
-    if (U / (seg + kAlignSlack) + BH / 2 <= int(gridDim.x)) {
+    if (ceil_div(U, seg + kAlignSlack) + BH / 2 <= int(gridDim.x)) {
       for (int more = 0; more <= kAlignSlack; more += more ? more : 2) {
         const int longer = seg + more;
-        int ctas = 0;
+        int cut[kLaneHeads], ctas = 0;
 #pragma unroll
-        for (int k = 0; k < kLaneHeads; ++k)
-          if (k < per) ctas += (n[k] + longer - 1) / longer;
+        for (int k = 0; k < kLaneHeads; ++k) {
+          cut[k] = 0;
+          if (k < per) cut[k] = ceil_div(n[k], longer);
+          ctas += cut[k];
+        }
         if (__reduce_add_sync(0xffffffff, ctas) > int(gridDim.x)) continue;
         seg = longer;
         sum = 0;
 #pragma unroll
         for (int k = 0; k < kLaneHeads; ++k) {
-          if (k < per) room[k] = (n[k] + seg - 1) / seg * seg;
+          room[k] = cut[k] * seg;
           sum += room[k];
         }
         break;
@@ -283,14 +298,18 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv4_decode_kernel(Kv4DecodePa
     const int per = (BH + kThreads - 1) / kThreads;
     const int i0 = min(BH, tid * per), i1 = min(BH, i0 + per);
     int sum = 0, U;
-    for (int i = i0; i < i1; ++i) sum += (head_len(p, i) + 15) >> 4;
+    for (int i = i0; i < i1; ++i) {
+      sum += (head_len(p, i) + 15) >> 4;
+      if (blockIdx.x == 0 && __ldg(p.seqlens + (i >> p.halves)) > p.c.width * p.c.page)
+        set_error(p.c.err, WGKV_ERR_HEAD_CAPACITY);
+    }
     int run = block_excl_scan<kThreads>(sum, scan, U);
     for (int i = i0; i < i1; ++i) {
       pre[i] = run;
       run += (head_len(p, i) + 15) >> 4;
       fin[i] = run;
     }
-    seg = max(kMinSegment, (U + int(gridDim.x) - 1) / int(gridDim.x));
+    seg = max(kMinSegment, ceil_div(U, gridDim.x));
     u0 = min(U, int(blockIdx.x) * seg);
     u1 = min(U, u0 + seg);
     __syncthreads();
@@ -303,10 +322,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv4_decode_kernel(Kv4DecodePa
     }
   }
   auto rows_of = [&](int bh) { return min(G, p.group - (bh & p.halves) * G); };  // query heads of head bh
-  for (int bh = blockIdx.x; bh < BH; bh += gridDim.x) {  // heads that hold nothing, lengths past the table
+  for (int bh = blockIdx.x; bh < BH; bh += gridDim.x) {  // heads that hold nothing
     if (fin[bh] == pre[bh])
       for (int e = tid; e < rows_of(bh) * D; e += kThreads) p.out[query_row(p, bh) * D + e] = 0;
-    if (tid == 0 && __ldg(p.seqlens + (bh >> p.halves)) > p.c.width * p.c.page) set_error(p.c.err, WGKV_ERR_HEAD_CAPACITY);
   }
   if (u0 >= u1) return;
 
@@ -929,7 +947,7 @@ extern "C" int wgkv_paged_decode_kv4(const uint16_t* q, const uint8_t* cache, in
       num_q_heads / num_kv_heads > kMaxG || int64_t(batch) * num_kv_heads > kMaxBH)
     return WGKV_EINVAL;
   if (num_pages <= 0 || page_size <= 0 || page_size % 16 || table_width <= 0 || table_stride < table_width ||
-      int64_t(batch) * num_kv_heads * table_width * (page_size / 16) >= (int64_t(1) << 30) ||
+      int64_t(batch) * num_kv_heads * table_width * (page_size / 16) >= (int64_t(1) << 29) ||
       int64_t(table_width) * page_size >= (int64_t(1) << 31) || num_pages * (page_size / 16) >= (int64_t(1) << 31) ||
       (reinterpret_cast<uintptr_t>(cache) & 15) || (reinterpret_cast<uintptr_t>(q) & 15) ||
       (reinterpret_cast<uintptr_t>(out) & 15) || (reinterpret_cast<uintptr_t>(workspace) & 255))
