@@ -30,6 +30,8 @@
  *   wgkv_snapkv_evict         snapkv_evict :595-671 (free list reused by promotion :694-709)
  *   wgkv_paged_decode         flash_attn_with_kvcache_wrapper_triton_handle + split/reduce kernels :818-1140
  *                             (and the batched flash_attn_with_kvcache_wrapper :766-811)
+ *   wgkv_kv4_*                (no reference counterpart) the pool, or any paged cache, held in 4 bits:
+ *   wgkv_paged_decode_kv4     writer, reader and decode attention
  *   wgkv_oproj_allreduce      self.o_proj(attn_output) (src/modeling_llama.py:286) of a KV-head-sharded
  *                             layer plus the sum over GPUs (the reference has no tensor parallelism)
  */
