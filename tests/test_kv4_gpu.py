@@ -422,6 +422,32 @@ def test_decode_graphs_and_streams(wgkv):
     assert torch.equal(third, want[2])
 
 
+def test_integers_past_32_bits_stay_out_of_range(wgkv):
+    rng = np.random.default_rng(16)
+    lens = np.array([[40, 33]], np.int32)
+    cache, tbl, hk, hv = filled(wgkv, rng, lens, 64, 32, 16)
+    before = cache.clone()
+    row = dev(kv_rows(rng, 1, 2, 1, 64))
+    far = torch.tensor([[2 ** 32, -2 ** 32 + 1]], device="cuda")
+    wgkv.kv4_append(row, row, cache, far, dev_i(tbl))
+    with pytest.raises(AssertionError, match="max_tokens_per_head"):
+        wgkv.check_errors()
+    assert torch.equal(cache, before)
+    q = K4.bf16(rng.standard_normal((1, 1, 4, 64)))
+    ln = torch.tensor([[40, 2 ** 32 + 5]], device="cuda")
+    out = wgkv.paged_decode_kv4(dev(q), cache, ln, dev_i(tbl), 0.125)
+    with pytest.raises(AssertionError, match="max_tokens_per_head"):
+        wgkv.check_errors()
+    want, tol = K4.decode(q, hk, hv, lens, 0.125)
+    within(out.double().cpu().numpy()[:, :, :2], want[:, :, :2], tol[:, :, :2])
+    bt = dev_i(tbl).long()
+    bt[0, 1, 0] += 2 ** 32
+    k, v = wgkv.kv4_read(cache, None, dev_i(lens), bt, 40)
+    with pytest.raises(AssertionError, match="page id out of range"):
+        wgkv.check_errors()
+    assert (k[0, 1, :16] == 0).all() and (v[0, 1, :16] == 0).all()
+
+
 # ------------------------------------------------------------------------------- as they are used together
 @pytest.mark.parametrize("D,group,T", [(128, 64, 16), (64, 32, 32)])
 def test_prompt_then_tokens(wgkv, D, group, T):

@@ -94,6 +94,8 @@ def _integers(t, name):
     if t.dtype is not _I32:
         if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype is torch.bool:
             raise TypeError(f"{name} must hold integers, got {t.dtype}")
+        if t.dtype is torch.int64:  # out of range stays out of range
+            t = t.clamp(-2 ** 31, 2 ** 31 - 1)
         t = t.to(_I32)
     return t
 
