@@ -549,7 +549,8 @@ WGKV_API int wgkv_kv4_read(const uint8_t* cache, int64_t num_pages, int page_siz
  * leaves that head's output undefined.  A head of length 0 (or below) yields zeros.  All sums and softmax
  * statistics are fp32; the probabilities, times V's scale, are rounded to fp16 before the PV product.
  * Constraints: (head_dim, group) as above; page_size % 16 == 0; Hq % Hk == 0; Hq / Hk <= 16;
- * B * Hk <= 4096; B * Hk * table_width * page_size / 16 < 2^29; 16-byte aligned q, out and cache.
+ * B * Hk <= 4096; B * Hk * table_width * page_size / 16 < 2^29 (2^28 if Hq / Hk > 8); 16-byte aligned q, out
+ * and cache.
  * workspace: wgkv_paged_decode_kv4_workspace_size() bytes, 256-byte aligned, its first B*Hk*8 bytes zero
  * before the first call (the kernel leaves them zero); calls sharing a workspace must be stream-ordered.
  */

@@ -237,3 +237,11 @@ def test_pool_refusals():
     assert _kv_group(SimpleNamespace(kv_cache_bits=4, kv_cache_group=32)) == 32
     with pytest.raises(ValueError):
         _kv_group(SimpleNamespace(kv_cache_bits=8))
+
+
+@needs_lib
+def test_decode_counts_the_records_of_divided_heads():
+    # more than 8 query heads on a KV head are worked on as two heads: half as many records fit
+    assert _decode(B=1024, Hk=4, Hq=32, width=(1 << 16) - 1, stride=1 << 16, page=32, nbytes=0) == ENOSPC
+    assert _decode(B=1024, Hk=4, Hq=36, width=(1 << 16) - 1, stride=1 << 16, page=32, nbytes=0) == EINVAL
+    assert _decode(B=1024, Hk=4, Hq=36, width=(1 << 15) - 1, stride=1 << 16, page=32, nbytes=0) == ENOSPC

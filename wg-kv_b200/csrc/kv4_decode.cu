@@ -201,7 +201,8 @@ WGKV_DEV int head_len(const Kv4DecodeParams& p, int bh) {
   return min(max(__ldg(p.seqlens + (bh >> p.halves)), 0), p.c.width * p.c.page);
 }
 
-// ceil(n / d) for 0 <= n < 2^30, d > 0: a quotient in fp32 is at most one off.
+// ceil(n / d) for 0 <= n < 2^29, d > 0 and a quotient below 2^21 (n over the CTAs, or below their number):
+// in fp32 it is at most one off.
 WGKV_DEV int ceil_div(int n, int d) {
   n += d - 1;
   int q = int(__fdividef(float(n), float(d)));
@@ -961,7 +962,8 @@ extern "C" int wgkv_paged_decode_kv4(const uint16_t* q, const uint8_t* cache, in
       num_q_heads / num_kv_heads > kMaxG || int64_t(batch) * num_kv_heads > kMaxBH)
     return WGKV_EINVAL;
   if (num_pages <= 0 || page_size <= 0 || page_size % 16 || table_width <= 0 || table_stride < table_width ||
-      int64_t(batch) * num_kv_heads * table_width * (page_size / 16) >= (int64_t(1) << 29) ||
+      (int64_t(batch) * num_kv_heads << head_halves(num_q_heads / num_kv_heads)) * table_width * (page_size / 16) >=
+          (int64_t(1) << 29) ||
       int64_t(table_width) * page_size >= (int64_t(1) << 31) || num_pages * (page_size / 16) >= (int64_t(1) << 31) ||
       (reinterpret_cast<uintptr_t>(cache) & 15) || (reinterpret_cast<uintptr_t>(q) & 15) ||
       (reinterpret_cast<uintptr_t>(out) & 15) || (reinterpret_cast<uintptr_t>(workspace) & 255))
