@@ -551,8 +551,9 @@ WGKV_API int wgkv_kv4_read(const uint8_t* cache, int64_t num_pages, int page_siz
  * Constraints: (head_dim, group) as above; page_size % 16 == 0; Hq % Hk == 0; Hq / Hk <= 16;
  * B * Hk <= 4096; B * Hk * table_width * page_size / 16 < 2^29 (2^28 if Hq / Hk > 8); 16-byte aligned q, out
  * and cache.
- * workspace: wgkv_paged_decode_kv4_workspace_size() bytes, 256-byte aligned, its first B*Hk*8 bytes zero
- * before the first call (the kernel leaves them zero); calls sharing a workspace must be stream-ordered.
+ * workspace: wgkv_paged_decode_kv4_workspace_size() bytes, 256-byte aligned, its first 32768 bytes zero
+ * before the first call (the kernel leaves them zero); calls sharing a workspace, of the same or of
+ * different sizes, must be stream-ordered.
  */
 WGKV_API size_t wgkv_paged_decode_kv4_workspace_size(int batch, int num_q_heads, int num_kv_heads, int head_dim);
 WGKV_API int wgkv_paged_decode_kv4(const uint16_t* q, const uint8_t* cache, int64_t num_pages, int page_size,

@@ -245,3 +245,10 @@ def test_decode_counts_the_records_of_divided_heads():
     assert _decode(B=1024, Hk=4, Hq=32, width=(1 << 16) - 1, stride=1 << 16, page=32, nbytes=0) == ENOSPC
     assert _decode(B=1024, Hk=4, Hq=36, width=(1 << 16) - 1, stride=1 << 16, page=32, nbytes=0) == EINVAL
     assert _decode(B=1024, Hk=4, Hq=36, width=(1 << 15) - 1, stride=1 << 16, page=32, nbytes=0) == ENOSPC
+
+
+@needs_lib
+def test_decode_workspace_holds_every_counter():
+    from wgkv import kv4
+    assert kv4._COUNTER_BYTES == 2 * 4096 * 4  # the most heads, twice for divided ones
+    assert lib.wgkv_paged_decode_kv4_workspace_size(1, 1, 1, 64) > kv4._COUNTER_BYTES

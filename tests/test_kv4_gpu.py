@@ -422,6 +422,31 @@ def test_decode_graphs_and_streams(wgkv):
     assert torch.equal(third, want[2])
 
 
+def test_decode_from_two_threads(wgkv):
+    """Calls of different sizes from two threads take turns in one stream's scratch."""
+    import threading
+    rng = np.random.default_rng(15)
+    cases = []
+    for lens, Hq, D in ((np.array([[9000, 5000]], np.int32), 8, 128),
+                        (rng.integers(1, 900, (24, 8)).astype(np.int32), 8, 64)):
+        cache, tbl, _, _ = filled(wgkv, rng, lens, D, 64, 16)
+        args = (dev(K4.bf16(rng.standard_normal((lens.shape[0], 1, Hq, D)))), cache, dev_i(lens), dev_i(tbl), D ** -0.5)
+        cases.append((args, wgkv.paged_decode_kv4(*args)))
+    wrong = []
+
+    def work(args, want):
+        for _ in range(200):
+            if not torch.equal(wgkv.paged_decode_kv4(*args), want):
+                wrong.append(1)
+
+    threads = [threading.Thread(target=work, args=c) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_integers_past_32_bits_stay_out_of_range(wgkv):
     rng = np.random.default_rng(16)
     lens = np.array([[40, 33]], np.int32)

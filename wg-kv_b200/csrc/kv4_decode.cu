@@ -884,17 +884,18 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv4_decode_kernel(Kv4DecodePa
 // one warp, whose registers leave 8 warps on an SM (26 us against 22 with 16 query heads, 141K tokens).
 int head_halves(int group) { return group > 8 ? 1 : 0; }
 
-size_t counter_bytes(int64_t BH) { return (size_t(BH) * 4 + 255) & ~size_t(255); }
+// One place for the counters whatever the number of heads: calls of different sizes may take turns in one
+// workspace without one's partial results lying where another counts.
+constexpr size_t kCounterBytes = 2 * kMaxBH * 4;
 
 size_t workspace_need(int64_t kv_heads, int group, int D, int sms) {
   const int halves = head_halves(group), G = (group + halves) >> halves;
   const int64_t BH = kv_heads << halves;
-  return counter_bytes(BH) + size_t(BH + sms * kCtas) * G * (D + 4) * 4 + 256;
+  return kCounterBytes + size_t(BH + sms * kCtas) * G * (D + 4) * 4 + 256;
 }
 
 struct DecodeLaunch {
   Kv4DecodeParams p;
-  void* ws;
   cudaStream_t stream;
   int sms, status;
   template <int D, int NG, int kPack>
@@ -982,7 +983,7 @@ extern "C" int wgkv_paged_decode_kv4(const uint16_t* q, const uint8_t* cache, in
   a.p.G = (group_heads + halves) >> halves;
   a.p.scale_log2 = softmax_scale * 1.4426950408889634f;
   a.p.counters = reinterpret_cast<int*>(workspace);
-  a.p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + counter_bytes(a.p.BH));
+  a.p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
   a.stream = as_stream(stream);
   a.sms = device_sms();
   if (a.sms <= 0) return WGKV_ECUDA;

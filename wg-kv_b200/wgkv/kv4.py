@@ -53,9 +53,10 @@ _APPEND_SLOTS, _READ_SLOTS, _DECODE_SLOTS = struct.Struct("=23q"), struct.Struct
 _append_plans: dict = {}
 _read_plans: dict = {}
 _decode_plans: dict = {}
-_scratch: dict = {}   # (device index, B, Hq, Hk, D) -> (workspace bytes, bytes of counters) of paged_decode_kv4
+_scratch: dict = {}   # (device index, B, Hq, Hk, D) -> workspace bytes of paged_decode_kv4
 _err_ptrs: dict = {}  # device index -> address of its error word
 _BF16, _I32 = torch.bfloat16, torch.int32
+_COUNTER_BYTES = 32768  # of paged_decode_kv4's workspace, zero between calls
 
 
 def _remember(plans, key, plan):
@@ -306,10 +307,9 @@ def paged_decode_kv4(q, cache, cache_seqlens, block_table, softmax_scale, out=No
     heads = (index, B, Hq, Hk, D)
     need = _scratch.get(heads)
     if need is None:
-        need = _remember(_scratch, heads, (int(lib.wgkv_paged_decode_kv4_workspace_size(B, Hq, Hk, D)),
-                                           (B * Hk * 8 + 255) // 256 * 256))
+        need = _remember(_scratch, heads, int(lib.wgkv_paged_decode_kv4_workspace_size(B, Hq, Hk, D)))
     stream = raw_stream(index)
-    ws, ws_bytes = counter_scratch(index, stream, "paged_decode_kv4", *need)
+    ws, ws_bytes = counter_scratch(index, stream, "paged_decode_kv4", need, _COUNTER_BYTES)
     _call(index, _DECODE,
           _DECODE_SLOTS.pack(q_ptr, cache.data_ptr(), pages, page, group, sl.data_ptr(), bt.data_ptr(), bt_rows, width,
                              B, Hq, Hk, D, softmax_scale, out.data_ptr(), ws, ws_bytes, _err_ptr(index), stream),

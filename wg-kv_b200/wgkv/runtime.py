@@ -74,28 +74,29 @@ def workspace(device, purpose: str, nbytes: int, zero_prefix: int = 0) -> torch.
     return ws
 
 
-_counter_scratch: dict = {}  # (device index, stream, purpose) -> [data pointer, bytes, zero prefix, tensor, capture id]
+_counter_scratch: dict = {}  # (device index, stream, purpose) -> (data pointer, bytes, capture id, tensors)
 
 
 def counter_scratch(index: int, stream: int, purpose: str, nbytes: int, zero_prefix: int):
-    """(pointer, bytes) of scratch of the current device whose first ``zero_prefix`` bytes are zero and are
-    left zero by the kernels that use it: :func:`workspace` for one raw stream, found with one dictionary
-    look-up, and safe under capture.  While a graph is captured its calls get scratch of the graph's own
-    (from its memory pool, zeroed by a node of the graph): graphs captured on one stream may replay on
-    several at a time, and must not share counters and partial results with one another or with the
-    stream's eager calls."""
+    """(pointer, bytes) of scratch of the current device whose first ``zero_prefix`` bytes (the same for every
+    call of a purpose) are zero and are left zero by the kernels that use it: :func:`workspace` for one raw
+    stream, found with one dictionary look-up, and safe under capture.  While a graph is captured its calls
+    get scratch of the graph's own (from its memory pool, zeroed by a node of the graph): graphs captured on
+    one stream may replay on several at a time, and must not share counters and partial results with one
+    another or with the stream's eager calls.  Scratch that was outgrown is kept (sizes double): another
+    thread may be about to launch on it."""
     capture = 0
     key = (index, stream, purpose)
     if torch.cuda.is_current_stream_capturing():
         capture = lib.wgkv_stream_capture_id(stream)
         key = (index, stream, purpose, "capture")
     ent = _counter_scratch.get(key)
-    if ent is None or ent[1] < nbytes or ent[4] != capture:
+    if ent is None or ent[1] < nbytes or ent[2] != capture:
+        nbytes = 1 << (nbytes - 1).bit_length()
         t = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
-        ent = _counter_scratch[key] = [t.data_ptr(), nbytes, 0, t, capture]
-    if ent[2] < zero_prefix:
-        ent[3][ent[2]:zero_prefix].zero_()  # stream-ordered, behind every earlier user on this stream
-    ent[2] = zero_prefix  # this call's kernels may write anything behind their own prefix
+        t[:zero_prefix].zero_()  # stream-ordered, before the first kernel that counts in it
+        outgrown = ent[3] if ent is not None and ent[2] == capture else ()
+        ent = _counter_scratch[key] = (t.data_ptr(), nbytes, capture, (*outgrown, t))
     return ent[0], ent[1]
 
 
