@@ -260,6 +260,23 @@ def test_decode_split_over_the_length(wgkv, D, group, Hq, Hk, B, longest):
     within(got, *K4.decode(q, hk, hv, lens, D ** -0.5))
 
 
+@pytest.mark.parametrize("D,group,Hq,Hk,B", [(64, 64, 16, 4, 50), (128, 32, 10, 2, 40), (64, 32, 20, 2, 30), (64, 64, 8, 8, 60)])
+def test_decode_many_unequal_heads(wgkv, D, group, Hq, Hk, B):
+    """Long heads between very short ones: a CTA's segment holds parts of several, and its warps run ahead of
+    one another where they end."""
+    rng = np.random.default_rng(17)
+    lens = rng.choice([0, 1, 16, 33, 70, 900, 5000], (B, Hk), p=[.1, .15, .15, .2, .1, .2, .1]).astype(np.int32)
+    cache, tbl, hk, hv = filled(wgkv, rng, lens, D, group, 16)
+    q = K4.bf16(rng.standard_normal((B, 1, Hq, D)))
+    args = dev(q), cache, dev_i(lens), dev_i(tbl), D ** -0.5
+    out = wgkv.paged_decode_kv4(*args)
+    again = [wgkv.paged_decode_kv4(*args) for _ in range(20)]
+    torch.cuda.synchronize()
+    wgkv.check_errors()
+    within(out.double().cpu().numpy(), *K4.decode(q, hk, hv, lens, D ** -0.5))
+    assert all(torch.equal(o, out) for o in again)
+
+
 @pytest.mark.parametrize("D,group,G", [(128, 64, 4), (64, 32, 8), (128, 128, 12)])
 def test_decode_long_flat_softmax_keeps_its_precision(wgkv, D, group, G):
     """Millions of records over V's that cancel: the result is hundreds of times smaller than the sums of
