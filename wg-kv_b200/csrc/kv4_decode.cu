@@ -54,7 +54,7 @@ namespace wgkv {
 namespace {
 
 constexpr int kNB = 2;         // records of a slot, which a warp works on together
-constexpr int kMaxSlots = 4;   // slots of a warp's ring
+constexpr int kMaxSlots = 2;   // slots of a warp's ring (3: 1-2 % slower at every size)
 constexpr int kLaneHeads = 8;  // heads per lane up to which a warp sums up all lengths itself
 constexpr int kMaxBH = 4096;
 constexpr int kMaxG = 16;
@@ -65,8 +65,10 @@ constexpr int kWarps = 6;
 constexpr int kCtas = 2;  // per SM
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMinSegment = kWarps * kNB;  // records a CTA gets at least
-// A CTA that meets a head's end spends about as long on the merge and the next head's start as on this
-// many records: segments are cut at the heads' ends where that makes them no longer than this.
+// A CTA that meets a head's end before its segment's spends about as long on the merge and the next head's
+// start as on kHeadCost records: the heads stand that far apart in the line.  Segments are cut at the heads'
+// ends where that makes them no more than kAlignSlack records longer.
+constexpr int kHeadCost = 40;
 constexpr int kAlignSlack = 16;
 
 struct Kv4DecodeParams {
@@ -265,17 +267,17 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv4_decode_kernel(Kv4DecodePa
       const int len = k < per && i < BH ? __ldg(p.seqlens + (i >> p.halves)) : 0;
       over |= len > p.c.width * p.c.page;
       n[k] = (min(max(len, 0), p.c.width * p.c.page) + 15) >> 4;
-      room[k] = n[k];
     }
     if (over && blockIdx.x == 0) set_error(p.c.err, WGKV_ERR_HEAD_CAPACITY);
 #pragma unroll
     for (int k = 0; k < kLaneHeads; ++k) sum += n[k];
     const int U = __reduce_add_sync(0xffffffff, sum);
-    seg = max(kMinSegment, ceil_div(U, gridDim.x));
+    const int least = max(kMinSegment, ceil_div(U, gridDim.x));
     // segments that end with the heads, if slightly longer ones are then few enough
-    if (ceil_div(U, seg + kAlignSlack) + BH / 2 <= int(gridDim.x)) {
+    seg = 0;
+    if (ceil_div(U, least + kAlignSlack) + BH / 2 <= int(gridDim.x)) {
       for (int more = 0; more <= kAlignSlack; more += more ? more : 2) {
-        const int longer = seg + more;
+        const int longer = least + more;
         int cut[kLaneHeads], ctas = 0;
 #pragma unroll
         for (int k = 0; k < kLaneHeads; ++k) {
@@ -293,6 +295,15 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv4_decode_kernel(Kv4DecodePa
         }
         break;
       }
+    }
+    if (seg == 0) {
+      sum = 0;
+#pragma unroll
+      for (int k = 0; k < kLaneHeads; ++k) {
+        room[k] = n[k] ? n[k] + kHeadCost : 0;
+        sum += room[k];
+      }
+      seg = max(kMinSegment, ceil_div(__reduce_add_sync(0xffffffff, sum), gridDim.x));
     }
     int run = sum;
 #pragma unroll
@@ -322,15 +333,17 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv4_decode_kernel(Kv4DecodePa
     const int i0 = min(BH, tid * per), i1 = min(BH, i0 + per);
     int sum = 0, U;
     for (int i = i0; i < i1; ++i) {
-      sum += (head_len(p, i) + 15) >> 4;
+      const int n = (head_len(p, i) + 15) >> 4;
+      sum += n ? n + kHeadCost : 0;
       if (blockIdx.x == 0 && __ldg(p.seqlens + (i >> p.halves)) > p.c.width * p.c.page)
         set_error(p.c.err, WGKV_ERR_HEAD_CAPACITY);
     }
     int run = block_excl_scan<kThreads>(sum, scan, U);
     for (int i = i0; i < i1; ++i) {
+      const int n = (head_len(p, i) + 15) >> 4;
       pre[i] = run;
-      run += (head_len(p, i) + 15) >> 4;
-      fin[i] = run;
+      fin[i] = run + n;
+      run += n ? n + kHeadCost : 0;
     }
     seg = max(kMinSegment, ceil_div(U, gridDim.x));
     u0 = min(U, int(blockIdx.x) * seg);
@@ -364,7 +377,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv4_decode_kernel(Kv4DecodePa
     for (int j = 0; j < W; ++j)
       raw_q[j] = head < rows_of(bh) ? __ldg(reinterpret_cast<const uint4*>(src + 32 * j)) : make_uint4(0, 0, 0, 0);
   };
-  while (fin[lo] <= u0) ++lo;  // past heads that hold nothing
+  while (lo < BH && fin[lo] <= max(u0, pre[lo])) ++lo;  // past heads that end before, or hold nothing
+  if (lo == BH || pre[lo] >= u1) return;
   load_q(lo);
 
   // ---- this warp's records in order: of the pairs of each head's part of the segment, every kWarps-th ----
@@ -670,9 +684,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv4_decode_kernel(Kv4DecodePa
       }
     };
 
-    // The scores of a pair are computed in one stretch of code with the weights and products of the one
-    // before, which do not depend on them; the part's last pair (one record, perhaps, and perhaps the head's
-    // end) goes by itself.
+    // The part's last pair (one record, perhaps, and perhaps the head's end) goes by itself.  (Taking a pair's
+    // scores in one stretch of code with the weights and products of the one before: 93 us against 91.)
     const int pairs = (re - rs + 1) >> 1;
     const int mine = (pairs - warp + kWarps - 1) / kWarps;                   // this warp's
     const int whole_pairs = mine - (mine > 0 && (pairs - 1) % kWarps == warp);
@@ -685,23 +698,12 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv4_decode_kernel(Kv4DecodePa
     };
     Scores x;
     float top[2];
-    if (whole_pairs > 0) {
-      uint32_t now = arrived();
+    for (int i = 0; i < whole_pairs; ++i) {
+      const uint32_t now = arrived();
       scores(now, Whole<true>(), kNB, 0, x, top);
       settle(x, top);
-      for (int i = 1; i < whole_pairs; ++i) {
-        const uint32_t next = arrived();
-        Scores y;
-        scores(next, Whole<true>(), kNB, 0, y, top);
-        weigh(now, Whole<true>(), kNB, 0, x);
-        __syncwarp();  // every lane has read the slot
-        issue();
-        settle(y, top);
-        x = y;
-        now = next;
-      }
       weigh(now, Whole<true>(), kNB, 0, x);
-      __syncwarp();
+      __syncwarp();  // every lane has read the slot
       issue();
     }
     if (mine > whole_pairs) {
