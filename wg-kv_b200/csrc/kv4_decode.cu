@@ -35,18 +35,22 @@
 //
 // Work is cut as in paged_decode.cu: the 16-token records of all heads laid end to end, equal segments per
 // CTA; a head cut over CTAs is merged by the last one to finish it (self-resetting counter, fixed order of
-// summation).  Inside a CTA every warp is on its own: it takes every kWarps-th pair of records of the
-// segment's part of a head, copies them itself (cp.async.bulk, one whole record each) into a ring of
-// slots of its own, a pair each, and works on a pair at a time; page ids are looked up 32 records at a
-// time, a batch ahead.  Warps meet only where a head ends.  (One producer warp for all, a stage shared by
-// all warps: 112 us against 102; the copies alone, without any arithmetic: 85 us.)
+// summation).  Heads stand apart in that line by what the end of one costs (kHeadCost): the CTAs with most
+// heads' ends in their segments had finished up to 20 % later than the others.  Inside a CTA every warp is on
+// its own: it takes every kWarps-th pair of records of the segment's part of a head, copies them itself
+// (cp.async.bulk, one whole record each) into a ring of slots of its own, a pair each, and works on a pair at a
+// time; page ids are looked up 32 records at a time, a batch ahead.  Warps meet only where a head ends.
+// Measured and not taken: one producer warp for all and a stage shared by all warps (112 us against 102 then);
+// one warp merging the states while the others go on with the next head (100 against 97); the join of partial
+// results fed by bulk copies into shared memory (25 against 21 us with 8 heads of 16 rows).  The copies alone,
+// without any arithmetic, take 85 us.
 //
-// Measured on B200: 3.5M tokens x KV heads (G = 4, D = 128, groups of 64, 504 MB) in 97 us, 5.2 TB/s, 0.79
-// of the copy bandwidth, 3 times as fast as the bf16 kernel on the same tokens (1.79 GB, 287 us).  What bounds it there is
-// issue: 230 instructions a record, 80 of them unpacking, at 0.52 of the issue slots with 3 warps per
-// scheduler (168 registers); integer pipe 0.55, tensor pipe 0.29.  A single sequence of 2K tokens takes
-// 9.6 us, all of it latency: four dependent look-ups (lengths, table, records; then the counter and the
-// partial results) of 0.4 to 1 us each around one pair of records per warp.
+// Measured on B200: 3.5M tokens x KV heads (G = 4, D = 128, groups of 64, 504 MB) in 91 us, 5.5 TB/s, 0.85
+// of the copy bandwidth, 3 times as fast as the bf16 kernel on the same tokens (1.79 GB, 287 us).  What bounds it
+// there is latency with 3 warps per scheduler (168 registers): 230 instructions a record, 80 of them unpacking, at
+// 0.55 of the issue slots and 0.58 of the integer pipe.  A single sequence of 2K tokens takes 8.8 us, all of it
+// latency: four dependent look-ups (lengths, table, records; then the counter and the partial results) of 0.4 to 1
+// us each around one pair of records per warp.
 #include "kv4.cuh"
 #include "runtime.h"
 
@@ -54,17 +58,16 @@ namespace wgkv {
 namespace {
 
 constexpr int kNB = 2;         // records of a slot, which a warp works on together
-constexpr int kMaxSlots = 2;   // slots of a warp's ring (3: 1-2 % slower at every size)
+constexpr int kSlots = 2;      // slots of a warp's ring (3: 1-2 % slower at every size)
 constexpr int kLaneHeads = 8;  // heads per lane up to which a warp sums up all lengths itself
 constexpr int kMaxBH = 4096;
 constexpr int kMaxG = 16;
 
-// 6 warps of 168 registers in two CTAs per SM.  8 warps of 128 spill (112 us against 97 at 3.5M tokens x
-// heads), 12 warps in one CTA all wait where a head ends (106 us).
-constexpr int kWarps = 6;
-constexpr int kCtas = 2;  // per SM
-constexpr int kThreads = 32 * kWarps;
-constexpr int kMinSegment = kWarps * kNB;  // records a CTA gets at least
+// 12 warps of 168 registers on an SM: 6 in each of two CTAs, and 4 in each of three where there are many heads,
+// whose ends a CTA of fewer warps gets over sooner (256 heads and more: 16 -> 15 us and 56 -> 54 us, 512: 17.4
+// -> 16.1 us and 70 -> 67 us; 32 heads: 11.5 -> 12.5 us, 40 -> 40.5 us).  16 warps of 128 registers spill (100 us
+// against 90.5 at 3.5M tokens x heads).
+constexpr int kSmWarps = 12, kManyHeads = 256;
 // A CTA that meets a head's end before its segment's spends about as long on the merge and the next head's
 // start as on kHeadCost records: the heads stand that far apart in the line.  Segments are cut at the heads'
 // ends where that makes them no more than kAlignSlack records longer.
@@ -79,7 +82,7 @@ struct Kv4DecodeParams {
   int group;      // query heads per KV head
   int halves;     // 1 where a KV head's query heads are worked on as two heads of up to 8 (else 0)
   int BH, G;      // heads worked on, query heads of each (one fewer in a second half, if group is odd)
-  int slots;
+  int slots;      // kSlots: as a constant it costs registers (91 -> 93 us at 3.5M tokens x heads)
   float scale_log2;
   float* part;    // partial results: (BH + CTAs) x G x (D + 4)
   int* counters;  // per head
@@ -201,9 +204,9 @@ WGKV_DEV void store_out(uint16_t* out, const float4& A, float L) {
   *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(A.x / L, A.y / L), pack_bf16x2(A.z / L, A.w / L));
 }
 
-size_t fixed_smem(int BH, int G, int D) {
-  return 128 + size_t(kWarps) * G * (D + 4) * 4 + kThreads * 32 + kWarps * kMaxSlots * 8 +
-         size_t(2 * BH + kThreads + 2 * kWarps) * 4 + 64;
+size_t fixed_smem(int warps, int BH, int G, int D) {
+  return 128 + size_t(warps) * (G * (D + 4) * 4 + 32 * 32 + kSlots * 8) +
+         size_t(2 * BH + (32 + 2) * warps) * 4 + 64;
 }
 
 // Tokens of head bh that count: not below 0, not past the table.
@@ -226,19 +229,22 @@ WGKV_DEV size_t query_row(const Kv4DecodeParams& p, int bh) {
 }
 
 // kPack: records whose scores share the 8 columns of a tile: 2 for up to 4 query heads, else 1.
-template <int D, int NG, int kPack>
-__global__ void __launch_bounds__(kThreads, kCtas) kv4_decode_kernel(Kv4DecodeParams p) {
+template <int D, int NG, int kPack, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, kSmWarps / kWarps) kv4_decode_kernel(Kv4DecodeParams p) {
+  constexpr int kThreads = 32 * kWarps;
+  constexpr int kMinSegment = kWarps * kNB;  // records a CTA gets at least
   using F = Kv4<D, NG>;
   constexpr int kSets = kNB / kPack;  // sets of columns that a pair of records fills
   constexpr int W = D / 32;
   constexpr int kMR = merge_row<D>();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stage_base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
-  const int R = p.slots, G = p.G, BH = p.BH;
+  const int R = p.slots;
+  const int G = p.G, BH = p.BH;
   float* merge = reinterpret_cast<float*>(stage_base + size_t(kWarps) * R * kNB * F::kRec);  // [kWarps][G][kMR]
   float* join = merge + kWarps * G * kMR;                                                  // [kThreads][8]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(join + kThreads * 8);                        // [kWarps][kMaxSlots]
-  int* pre = reinterpret_cast<int*>(bars + kWarps * kMaxSlots);  // [BH] a head's first record in the line
+  uint64_t* bars = reinterpret_cast<uint64_t*>(join + kThreads * 8);                        // [kWarps][kSlots]
+  int* pre = reinterpret_cast<int*>(bars + kWarps * kSlots);  // [BH] a head's first record in the line
   int* fin = pre + BH;                                           // [BH] the one behind its last
   int* scan = fin + BH;                                          // [kThreads]
   int* flag = scan + kThreads + 2 * kWarps;
@@ -247,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv4_decode_kernel(Kv4DecodePa
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffff, tid >> 5, 0);  // the same in all lanes, so branches on it are uniform
   const uint32_t ring = smem_u32(stage_base) + warp * R * kNB * F::kRec;
-  uint64_t* full = bars + warp * kMaxSlots;
+  uint64_t* full = bars + warp * kSlots;
   if (lane < R) mbar_init(&full[lane], kNB);
   fence_barrier_init();
   *gave_up = 0;
@@ -272,7 +278,15 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv4_decode_kernel(Kv4DecodePa
 #pragma unroll
     for (int k = 0; k < kLaneHeads; ++k) sum += n[k];
     const int U = __reduce_add_sync(0xffffffff, sum);
-    const int least = max(kMinSegment, ceil_div(U, gridDim.x));
+    int longest = 0;
+#pragma unroll
+    for (int k = 0; k < kLaneHeads; ++k) longest = max(longest, n[k]);
+    longest = __reduce_max_sync(0xffffffff, longest);
+    // A partial result of G x D values costs the CTA that joins them about as long as G x D / 900 records: as
+    // many records to a segment, at least, as the partial results of the longest head are worth (2 KV heads of
+    // 8 query heads, 16K tokens: 20.8 -> 15.1 us).
+    const int worth = int(sqrtf(float(longest) * float(G * D) * (1.f / 900.f)));
+    const int least = max(max(kMinSegment, worth), ceil_div(U, gridDim.x));
     // segments that end with the heads, if slightly longer ones are then few enough
     seg = 0;
     if (ceil_div(U, least + kAlignSlack) + BH / 2 <= int(gridDim.x)) {
@@ -303,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv4_decode_kernel(Kv4DecodePa
         room[k] = n[k] ? n[k] + kHeadCost : 0;
         sum += room[k];
       }
-      seg = max(kMinSegment, ceil_div(__reduce_add_sync(0xffffffff, sum), gridDim.x));
+      seg = max(least, ceil_div(__reduce_add_sync(0xffffffff, sum), gridDim.x));
     }
     int run = sum;
 #pragma unroll
@@ -899,32 +913,25 @@ constexpr size_t kCounterBytes = 2 * kMaxBH * 4;
 size_t workspace_need(int64_t kv_heads, int group, int D, int sms) {
   const int halves = head_halves(group), G = (group + halves) >> halves;
   const int64_t BH = kv_heads << halves;
-  return kCounterBytes + size_t(BH + sms * kCtas) * G * (D + 4) * 4 + 256;
+  return kCounterBytes + size_t(BH + sms * (kSmWarps / 4)) * G * (D + 4) * 4 + 256;
 }
 
 struct DecodeLaunch {
   Kv4DecodeParams p;
   cudaStream_t stream;
   int sms, status;
-  template <int D, int NG, int kPack>
+  template <int D, int NG, int kPack, int kWarps>
   void launch() {
-    const size_t slot = size_t(kWarps) * kNB * Kv4<D, NG>::kRec;  // one more slot for every warp
-    const size_t fixed = fixed_smem(p.BH, p.G, D);
-    // As many slots as fit next to another CTA; with many heads or a large group (their prefix sums and
-    // merge rows) a CTA has the SM to itself.
-    size_t room = 227 * 1024 / kCtas - 1024;
-    if (fixed + 2 * slot > room) room = 227 * 1024;
-    if (fixed + 2 * slot > room) {
-      status = WGKV_EINVAL;
-      return;
-    }
-    p.slots = int((room - fixed) / slot < size_t(kMaxSlots) ? (room - fixed) / slot : size_t(kMaxSlots));
+    constexpr int kCtas = kSmWarps / kWarps;
+    const auto kernel = kv4_decode_kernel<D, NG, kPack, kWarps>;
+    // at most 128 KB: 8192 heads' places in the line
+    const size_t smem = fixed_smem(kWarps, p.BH, p.G, D) + size_t(kWarps) * kSlots * kNB * Kv4<D, NG>::kRec;
+    p.slots = kSlots;
     static bool attr_set[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 64 || !attr_set[dev]) {
-      if (cudaFuncSetAttribute(kv4_decode_kernel<D, NG, kPack>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               227 * 1024) != cudaSuccess) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) {
         status = WGKV_ECUDA;
         return;
       }
@@ -932,20 +939,25 @@ struct DecodeLaunch {
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(sms * kCtas);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = fixed + p.slots * slot;
+    cfg.blockDim = dim3(32 * kWarps);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // set-up overlaps the launch before
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    status = cudaLaunchKernelEx(&cfg, kv4_decode_kernel<D, NG, kPack>, p) == cudaSuccess ? WGKV_OK : WGKV_ECUDA;
+    status = cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? WGKV_OK : WGKV_ECUDA;
+  }
+  template <int D, int NG, int kPack>
+  void warps() {
+    if (p.BH >= kManyHeads) launch<D, NG, kPack, 4>();
+    else launch<D, NG, kPack, 6>();
   }
   template <int D, int NG>
   void run() {
-    if (p.G <= 4) launch<D, NG, 2>();
-    else launch<D, NG, 1>();
+    if (p.G <= 4) warps<D, NG, 2>();
+    else warps<D, NG, 1>();
   }
 };
 
