@@ -260,7 +260,8 @@ def test_decode_split_over_the_length(wgkv, D, group, Hq, Hk, B, longest):
     within(got, *K4.decode(q, hk, hv, lens, D ** -0.5))
 
 
-@pytest.mark.parametrize("D,group,Hq,Hk,B", [(64, 64, 16, 4, 50), (128, 32, 10, 2, 40), (64, 32, 20, 2, 30), (64, 64, 8, 8, 60)])
+@pytest.mark.parametrize("D,group,Hq,Hk,B", [(64, 64, 16, 4, 50), (128, 32, 10, 2, 40), (64, 32, 20, 2, 30), (64, 64, 8, 8, 60),
+                                             (64, 32, 48, 8, 40), (128, 128, 16, 1, 150)])
 def test_decode_many_unequal_heads(wgkv, D, group, Hq, Hk, B):
     """Long heads between very short ones: a CTA's segment holds parts of several, and its warps run ahead of
     one another where they end."""

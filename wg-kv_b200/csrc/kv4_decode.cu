@@ -65,9 +65,11 @@ constexpr int kMaxG = 16;
 
 // 12 warps of 168 registers on an SM: 6 in each of two CTAs, and 4 in each of three where there are many heads,
 // whose ends a CTA of fewer warps gets over sooner (256 heads and more: 16 -> 15 us and 56 -> 54 us, 512: 17.4
-// -> 16.1 us and 70 -> 67 us; 32 heads: 11.5 -> 12.5 us, 40 -> 40.5 us).  16 warps of 128 registers spill (100 us
-// against 90.5 at 3.5M tokens x heads).
-constexpr int kSmWarps = 12, kManyHeads = 256;
+// -> 16.1 us and 70 -> 67 us; 32 heads: 11.5 -> 12.5 us, 40 -> 40.5 us), and all in one where there are few heads
+// of more than 4 rows, whose partial results are then half as many (2 heads, 16K tokens: 15.1 -> 12.3 us, 16 heads,
+// 30K: 21.0 -> 18.8 us; 64 heads, 4K: 14.3 -> 14.5 us; with up to 4 rows 8 heads of 2K: 8.7 -> 9.7 us).  16 warps of
+// 128 registers spill (100 us against 90.5 at 3.5M tokens x heads).
+constexpr int kSmWarps = 12, kManyHeads = 256, kFewHeads = 64;
 // A CTA that meets a head's end before its segment's spends about as long on the merge and the next head's
 // start as on kHeadCost records: the heads stand that far apart in the line.  Segments are cut at the heads'
 // ends where that makes them no more than kAlignSlack records longer.
@@ -924,7 +926,7 @@ struct DecodeLaunch {
   void launch() {
     constexpr int kCtas = kSmWarps / kWarps;
     const auto kernel = kv4_decode_kernel<D, NG, kPack, kWarps>;
-    // at most 128 KB: 8192 heads' places in the line
+    // at most 128 KB, 8192 heads' places in the line among them, or 190 KB of 12 warps
     const size_t smem = fixed_smem(kWarps, p.BH, p.G, D) + size_t(kWarps) * kSlots * kNB * Kv4<D, NG>::kRec;
     p.slots = kSlots;
     static bool attr_set[64] = {false};
@@ -951,8 +953,10 @@ struct DecodeLaunch {
   }
   template <int D, int NG, int kPack>
   void warps() {
-    if (p.BH >= kManyHeads) launch<D, NG, kPack, 4>();
-    else launch<D, NG, kPack, 6>();
+    if (p.BH >= kManyHeads) return launch<D, NG, kPack, 4>();
+    if constexpr (kPack == 1)
+      if (p.BH < kFewHeads) return launch<D, NG, kPack, 12>();
+    launch<D, NG, kPack, 6>();
   }
   template <int D, int NG>
   void run() {
