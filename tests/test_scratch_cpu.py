@@ -1,0 +1,80 @@
+"""Scratch and error words that several threads ask for at once, with a stand-in for torch's allocator: whoever
+gets an address gets memory that stays."""
+import gc
+import threading
+import weakref
+from types import SimpleNamespace
+
+import pytest
+
+from wgkv import runtime
+
+
+class Block:
+    """Stands for a CUDA tensor: an address of its own for as long as it lives."""
+    live = weakref.WeakSet()
+
+    def __init__(self, n):
+        self.n = n
+        Block.live.add(self)
+
+    def data_ptr(self):
+        return id(self)
+
+    def __getitem__(self, _):
+        return self
+
+    def zero_(self):
+        return self
+
+
+def overlapping(monkeypatch, first_wait=0.5):
+    """Lets two allocations of different threads overlap if the code under test allows it: the first to come
+    waits for a second for a while, as it may when the allocator gives up the interpreter's lock."""
+    second, lock, seen = threading.Event(), threading.Lock(), []
+
+    def allocate(n, **_):
+        with lock:
+            seen.append(n)
+            mine = len(seen)
+        if mine == 1:
+            second.wait(first_wait)
+        else:
+            second.set()
+        return Block(n)
+
+    stand_in = SimpleNamespace(
+        empty=allocate, zeros=allocate, uint8="uint8", int32="int32", device=lambda *a: SimpleNamespace(index=a[-1]),
+        cuda=SimpleNamespace(is_current_stream_capturing=lambda: False, current_device=lambda: 0))
+    monkeypatch.setattr(runtime, "torch", stand_in)
+    return seen
+
+
+def from_threads(calls):
+    out = [None] * len(calls)
+
+    def work(i):
+        out[i] = calls[i]()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    gc.collect()
+    return out
+
+
+@pytest.mark.parametrize("before,sizes", [(None, (1000, 1000)), (None, (1000, 70000)), (500, (2000, 2000)),
+                                          (500, (70000, 1000))])
+def test_counter_scratch_of_two_threads_stays_allocated(monkeypatch, before, sizes):
+    monkeypatch.setattr(runtime, "_counter_scratch", {})
+    if before is not None:  # both threads outgrow what there is
+        overlapping(monkeypatch, 0.0)
+        runtime.counter_scratch(0, 7, "purpose", before, 256)
+    overlapping(monkeypatch)
+    got = from_threads([lambda n=n: runtime.counter_scratch(0, 7, "purpose", n, 256) for n in sizes])
+    alive = {b.data_ptr(): b.n for b in Block.live}
+    for (ptr, nbytes), need in zip(got, sizes):
+        assert ptr in alive, "an address was handed out whose memory has no owner"
+        assert alive[ptr] >= nbytes >= need

@@ -9,10 +9,13 @@ After a call only its own prefix is known to be zero.
 """
 from __future__ import annotations
 
+import threading
+
 import torch
 
 from ._lib import ERR_BITS, lib
 
+_lock = threading.Lock()  # held while something that outlives a call is made, not while it is looked up
 _err_words: dict = {}
 _workspaces: dict = {}
 
@@ -84,7 +87,9 @@ def counter_scratch(index: int, stream: int, purpose: str, nbytes: int, zero_pre
     get scratch of the graph's own (from its memory pool, zeroed by a node of the graph): graphs captured on
     one stream may replay on several at a time, and must not share counters and partial results with one
     another or with the stream's eager calls.  Scratch that was outgrown is kept (sizes double): another
-    thread may be about to launch on it."""
+    thread may be about to launch on it.  For the same reason a miss is served under a lock: of two threads
+    that miss together the second takes what the first has made, so that no address is handed out whose
+    tensor the dictionary does not hold."""
     capture = 0
     key = (index, stream, purpose)
     if torch.cuda.is_current_stream_capturing():
@@ -92,11 +97,14 @@ def counter_scratch(index: int, stream: int, purpose: str, nbytes: int, zero_pre
         key = (index, stream, purpose, "capture")
     ent = _counter_scratch.get(key)
     if ent is None or ent[1] < nbytes or ent[2] != capture:
-        nbytes = 1 << (nbytes - 1).bit_length()
-        t = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
-        t[:zero_prefix].zero_()  # stream-ordered, before the first kernel that counts in it
-        outgrown = ent[3] if ent is not None and ent[2] == capture else ()
-        ent = _counter_scratch[key] = (t.data_ptr(), nbytes, capture, (*outgrown, t))
+        with _lock:
+            ent = _counter_scratch.get(key)
+            if ent is None or ent[1] < nbytes or ent[2] != capture:
+                size = 1 << (nbytes - 1).bit_length()
+                t = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", index))
+                t[:zero_prefix].zero_()  # stream-ordered, before the first kernel that counts in it
+                outgrown = ent[3] if ent is not None and ent[2] == capture else ()
+                ent = _counter_scratch[key] = (t.data_ptr(), size, capture, (*outgrown, t))
     return ent[0], ent[1]
 
 
