@@ -6,8 +6,9 @@ import weakref
 from types import SimpleNamespace
 
 import pytest
+import torch
 
-from wgkv import runtime
+from wgkv import kv4, runtime
 
 
 class Block:
@@ -44,8 +45,8 @@ def overlapping(monkeypatch, first_wait=0.5):
         return Block(n)
 
     stand_in = SimpleNamespace(
-        empty=allocate, zeros=allocate, uint8="uint8", int32="int32", device=lambda *a: SimpleNamespace(index=a[-1]),
-        cuda=SimpleNamespace(is_current_stream_capturing=lambda: False, current_device=lambda: 0))
+        empty=allocate, zeros=allocate, uint8="uint8", int32="int32", device=torch.device, cuda=SimpleNamespace(
+            is_current_stream_capturing=lambda: False, current_device=lambda: 0))
     monkeypatch.setattr(runtime, "torch", stand_in)
     return seen
 
@@ -78,3 +79,23 @@ def test_counter_scratch_of_two_threads_stays_allocated(monkeypatch, before, siz
     for (ptr, nbytes), need in zip(got, sizes):
         assert ptr in alive, "an address was handed out whose memory has no owner"
         assert alive[ptr] >= nbytes >= need
+
+
+def test_error_word_of_two_threads_is_one(monkeypatch):
+    monkeypatch.setattr(runtime, "_err_words", {})
+    monkeypatch.setattr(kv4, "_err_ptrs", {})
+    seen = overlapping(monkeypatch)
+    got = from_threads([lambda: kv4._err_ptr(0), lambda: runtime.err_word("cuda:0").data_ptr(), lambda: kv4._err_ptr(0)])
+    word = runtime.err_word("cuda:0").data_ptr()  # what check_errors() reads
+    assert got == [word] * 3 and kv4._err_ptr(0) == word and len(seen) == 1
+
+
+def test_error_word_outlives_its_dictionary_entry(monkeypatch):
+    """An address that kernels are given for good belongs to memory that stays for good."""
+    monkeypatch.setattr(runtime, "_err_words", {})
+    monkeypatch.setattr(kv4, "_err_ptrs", {})
+    overlapping(monkeypatch, 0.0)
+    ptr = kv4._err_ptr(0)
+    runtime._err_words.clear()
+    gc.collect()
+    assert ptr in {b.data_ptr() for b in Block.live}

@@ -54,7 +54,7 @@ _append_plans: dict = {}
 _read_plans: dict = {}
 _decode_plans: dict = {}
 _scratch: dict = {}   # (device index, B, Hq, Hk, D) -> workspace bytes of paged_decode_kv4
-_err_ptrs: dict = {}  # device index -> address of its error word
+_err_ptrs: dict = {}  # device index -> (address of its error word, the word)
 _BF16, _I32 = torch.bfloat16, torch.int32
 _COUNTER_BYTES = 32768  # of paged_decode_kv4's workspace, zero between calls
 
@@ -144,8 +144,9 @@ def _call(index, op, slots, what, B, Hk, width, cache):
 def _err_ptr(index):
     p = _err_ptrs.get(index)
     if p is None:
-        p = _err_ptrs[index] = err_word(torch.device("cuda", index)).data_ptr()
-    return p
+        word = err_word(torch.device("cuda", index))
+        p = _err_ptrs[index] = word.data_ptr(), word
+    return p[0]
 
 
 def _append_plan(k, v, cache, start, block_table, counts):

@@ -39,8 +39,10 @@ def err_word(device) -> torch.Tensor:
     key = d.index if d.index is not None else torch.cuda.current_device()
     w = _err_words.get(key)
     if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
-        _err_words[key] = w
+        with _lock:  # one word a device, whichever threads ask first: check_errors() reads no other
+            w = _err_words.get(key)
+            if w is None:
+                w = _err_words[key] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
     return w
 
 
