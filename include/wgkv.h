@@ -578,6 +578,13 @@ WGKV_API int wgkv_kv4_call(int op, const void* slots);
  */
 WGKV_API uint64_t wgkv_stream_capture_id(void* stream);
 
+/*
+ * Sets the calling thread's stream capture mode (0 global, 1 thread-local, 2 relaxed) and returns the one
+ * before it, or WGKV_EINVAL / WGKV_ECUDA.  Relaxed, the thread may allocate while it captures a stream:
+ * what outlives a graph must not lie in the graph's memory.
+ */
+WGKV_API int wgkv_thread_capture_mode(int mode);
+
 #ifdef __cplusplus
 }
 #endif

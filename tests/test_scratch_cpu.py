@@ -1,6 +1,8 @@
 """Scratch and error words that several threads ask for at once, with a stand-in for torch's allocator: whoever
 gets an address gets memory that stays."""
+import contextlib
 import gc
+import os
 import threading
 import weakref
 from types import SimpleNamespace
@@ -9,6 +11,7 @@ import pytest
 import torch
 
 from wgkv import kv4, runtime
+from wgkv._lib import LIB_PATH, lib
 
 
 class Block:
@@ -46,9 +49,20 @@ def overlapping(monkeypatch, first_wait=0.5):
 
     stand_in = SimpleNamespace(
         empty=allocate, zeros=allocate, uint8="uint8", int32="int32", device=torch.device, cuda=SimpleNamespace(
-            is_current_stream_capturing=lambda: False, current_device=lambda: 0))
+            is_current_stream_capturing=lambda: False, current_device=lambda: 0, Stream=lambda: Stream(1),
+            stream=lambda s: contextlib.nullcontext(), device=lambda d: contextlib.nullcontext()))
     monkeypatch.setattr(runtime, "torch", stand_in)
+    monkeypatch.setattr(runtime, "lib", SimpleNamespace(wgkv_thread_capture_mode=lambda m: 0,
+                                                        wgkv_stream_capture_id=lambda s: 0))
     return seen
+
+
+class Stream:
+    def __init__(self, raw):
+        self.cuda_stream, self.waited = raw, False
+
+    def synchronize(self):
+        self.waited = True
 
 
 def from_threads(calls):
@@ -99,3 +113,42 @@ def test_error_word_outlives_its_dictionary_entry(monkeypatch):
     runtime._err_words.clear()
     gc.collect()
     assert ptr in {b.data_ptr() for b in Block.live}
+
+
+@pytest.mark.parametrize("fails", [False, True])
+def test_error_word_is_made_outside_of_captures(monkeypatch, fails):
+    """On a stream that is not capturing (torch deals its streams in turns), waited for, and with the thread's
+    capture mode put back whatever happens."""
+    monkeypatch.setattr(runtime, "_err_words", {})
+    overlapping(monkeypatch, 0.0)
+    mode, streams, inside = [0], [Stream(5), Stream(5), Stream(6)], []
+
+    def exchange(m):
+        mode[0], old = m, mode[0]
+        return old
+
+    @contextlib.contextmanager
+    def current(s):
+        inside.append((s.cuda_stream, mode[0]))
+        yield
+        if fails:
+            raise MemoryError
+
+    dealt = iter(streams)
+    monkeypatch.setattr(runtime, "lib", SimpleNamespace(wgkv_thread_capture_mode=exchange,
+                                                        wgkv_stream_capture_id=lambda s: 77 if s == 5 else 0))
+    monkeypatch.setattr(runtime.torch.cuda, "Stream", lambda: next(dealt))
+    monkeypatch.setattr(runtime.torch.cuda, "stream", current)
+    if fails:
+        with pytest.raises(MemoryError):
+            runtime.err_word("cuda:0")
+        assert not runtime._err_words
+    else:
+        runtime.err_word("cuda:0")
+        assert streams[2].waited
+    assert inside == [(6, 2)] and mode == [0]
+
+
+@pytest.mark.skipif(not os.path.exists(LIB_PATH), reason="libwgkv.so not built")
+def test_capture_mode_is_checked():
+    assert lib.wgkv_thread_capture_mode(3) == -1 and lib.wgkv_thread_capture_mode(-1) == -1

@@ -67,3 +67,12 @@ int device_sms() {
 extern "C" int wgkv_version(void) { return 1; }
 
 extern "C" int wgkv_num_sms(void) { return wgkv::device_sms(); }
+
+extern "C" int wgkv_thread_capture_mode(int mode) {
+  if (mode < 0 || mode > 2) return WGKV_EINVAL;
+  cudaStreamCaptureMode m = mode == 0   ? cudaStreamCaptureModeGlobal
+                            : mode == 1 ? cudaStreamCaptureModeThreadLocal
+                                        : cudaStreamCaptureModeRelaxed;
+  if (cudaThreadExchangeStreamCaptureMode(&m) != cudaSuccess) return WGKV_ECUDA;
+  return m == cudaStreamCaptureModeGlobal ? 0 : m == cudaStreamCaptureModeThreadLocal ? 1 : 2;
+}

@@ -13,7 +13,7 @@ import threading
 
 import torch
 
-from ._lib import ERR_BITS, lib
+from ._lib import ERR_BITS, check, lib
 
 _lock = threading.Lock()  # held while something that outlives a call is made, not while it is looked up
 _err_words: dict = {}
@@ -34,6 +34,27 @@ def stream_ptr(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _new_error_word(index: int) -> torch.Tensor:
+    """A zero on device ``index`` that kernels of any stream may flag from now on.
+
+    It is made on a stream of its own and waited for: the current stream may have work queued behind which
+    the zero would arrive after another stream's flag, or may be capturing a graph, in whose memory the word
+    would be set to zero by every replay."""
+    mode = lib.wgkv_thread_capture_mode(2)
+    check(min(mode, 0), "wgkv_thread_capture_mode")
+    try:
+        with torch.cuda.device(index):
+            stream = torch.cuda.Stream()
+            while lib.wgkv_stream_capture_id(stream.cuda_stream):  # torch deals its streams in turns
+                stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                w = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+            stream.synchronize()
+    finally:
+        lib.wgkv_thread_capture_mode(mode)
+    return w
+
+
 def err_word(device) -> torch.Tensor:
     d = torch.device(device)
     key = d.index if d.index is not None else torch.cuda.current_device()
@@ -42,7 +63,7 @@ def err_word(device) -> torch.Tensor:
         with _lock:  # one word a device, whichever threads ask first: check_errors() reads no other
             w = _err_words.get(key)
             if w is None:
-                w = _err_words[key] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
+                w = _err_words[key] = _new_error_word(key)
     return w
 
 
