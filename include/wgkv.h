@@ -547,7 +547,10 @@ WGKV_API int wgkv_kv4_read(const uint8_t* cache, int64_t num_pages, int page_siz
  * those that the cache stands for (unrounded).  A length past the table's pages flags
  * WGKV_ERR_HEAD_CAPACITY and is cut there; a page id outside [0, num_pages) flags WGKV_ERR_BAD_PAGE and
  * leaves that head's output undefined.  A head of length 0 (or below) yields zeros.  All sums and softmax
- * statistics are fp32; the probabilities, times V's scale, are rounded to fp16 before the PV product.
+ * statistics are fp32; the probabilities, times V's scale, are rounded to fp16 before the PV product: to 11
+ * bits while they are within 2^-20 of a head's largest such weight (over all groups of its tokens), and by no
+ * more than 2^-31 of that largest weight below.  So the tail behind a heavy token, or a group whose scales are
+ * far below those of another group of the same rows, is held to full precision down to that distance.
  * Constraints: (head_dim, group) as above; page_size % 16 == 0; Hq % Hk == 0; Hq / Hk <= 16;
  * B * Hk <= 4096; B * Hk * table_width * page_size / 16 < 2^29 (2^28 if Hq / Hk > 8); 16-byte aligned q, out
  * and cache.

@@ -16,10 +16,15 @@
 //   sums are subtracted at the end (in fp32, 17 times the low codes' rounding).
 // * q enters as fp16 times a power of two per head that puts its largest element in [2^14, 2^15): exact
 //   down to 2^-24 of it, 2^-36 of it absolute below.
-// * The weights p s_v are rounded to fp16 (11 bits).  The reference 2^r of p is a running maximum over
-//   x + exponent(s_v), not over x, so that the weights, not the probabilities, are near 1 however V's
-//   scale differs between tokens; it moves only when a weight would pass 2^9.  Exponents below -40 count
-//   as -40.  Sums of p and p m_v stay fp32.
+// * The weights p s_v are rounded to fp16: to 11 bits from 2^-14 up, to multiples of 2^-24 below.  The
+//   reference 2^r of p is a running maximum over x + exponent(s_v), not over x, so that the weights, not the
+//   probabilities, have the same largest size however V's scale differs between tokens.  It is the token's
+//   largest scale that counts, so the weights of a group with smaller scales, and those of a long tail behind
+//   one heavy token, lie below: the largest weight is settled at 2^7 and the reference moves only when one
+//   would pass 2^15.5, near the end of fp16's range, which leaves 20 bits below the largest weight for the
+//   smaller ones to be normal numbers in, and 31 until they vanish (settled at 1, 7 fewer, groups 2^-12 apart
+//   behind a token 8 nats above the rest were lost).  Exponents below -40 count as -40.  Sums of p
+//   and p m_v stay fp32.
 // * The tensor cores' fp32 accumulation truncates.  Sums of codes, all positive, lose up to 2^-23 of
 //   themselves with every record added, and V's that cancel (any long, flat softmax) leave a result
 //   hundreds of times smaller than the sums: 8e-3 of it was lost at 28K tokens.  So every record's (or
@@ -75,6 +80,10 @@ constexpr int kSmWarps = 12, kManyHeads = 256, kFewHeads = 64;
 // ends where that makes them no more than kAlignSlack records longer.
 constexpr int kHeadCost = 40;
 constexpr int kAlignSlack = 16;
+// Exponents (of two) of the weights: where the largest is settled, and which one moves the reference.  A weight is
+// below 2^1.5 times what its exponent says (scales up to 2, the exponent's sum rounded to an integer), and fp16
+// ends at 2^16.
+constexpr float kSettled = 7.f, kLargest = 14.f;
 
 struct Kv4DecodeParams {
   Kv4Pages c;
@@ -601,7 +610,7 @@ __global__ void __launch_bounds__(32 * kWarps, kSmWarps / kWarps) kv4_decode_ker
     };
     // Moves the reference where a weight would outgrow it: most pairs only learn that none does.
     auto settle = [&](Scores& x, const float (&top)[2]) {
-      if (__any_sync(0xffffffff, first || fmaxf(top[0], top[1]) > 8388608.f + 127.f + 8.f)) {
+      if (__any_sync(0xffffffff, first || fmaxf(top[0], top[1]) > 8388608.f + 127.f + kLargest)) {
         float fac[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -609,7 +618,7 @@ __global__ void __launch_bounds__(32 * kWarps, kSmWarps / kWarps) kv4_decode_ker
           m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 4));
           m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 8));
           m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 16));
-          m -= 8388608.f + 127.f;
+          m -= 8388608.f + 127.f + kSettled;
           // up by `by`, where that is positive; the first time to where it belongs (a floor keeps it finite)
           const float by = fmaxf(m, first ? -1e30f : 0.f);
           const float f = first ? 0.f : exp2_approx(-by);
