@@ -537,6 +537,20 @@ __global__ void __launch_bounds__(32 * kWarps, kSmWarps / kWarps) kv4_decode_ker
     struct Scores {
       float v[kSets][4];
     };
+    // 2^23 + biased exponent of the largest scale of the V rows (at least -40) of tokens g and g + 8: added to x
+    // it rounds it to an integer, close enough for a bound
+    auto exponents = [&](uint32_t rec) {
+      uint32_t vp0[NG], vp1[NG];
+      lds_words<NG>(vp0, rec + F::kVP + g * 4 * NG);
+      lds_words<NG>(vp1, rec + F::kVP + (g + 8) * 4 * NG);
+      uint32_t v0 = uint32_t(127 - 40) << 23, v1 = v0;
+#pragma unroll
+      for (int n2 = 0; n2 < NG; ++n2) {
+        v0 = max(v0, vp0[n2]);
+        v1 = max(v1, vp1[n2]);
+      }
+      return make_float2(__uint_as_float(0x4b000000u | v0 >> 23), __uint_as_float(0x4b000000u | v1 >> 23));
+    };
     // Scores of a pair of records relative to the reference, and a bound of their weights.  kAll: both are
     // there and every token counts, so that nothing branches.
     auto scores = [&](uint32_t recs, auto all, int nb, int left, Scores& x, float (&top)[2]) {
@@ -544,7 +558,10 @@ __global__ void __launch_bounds__(32 * kWarps, kSmWarps / kWarps) kv4_decode_ker
       top[0] = top[1] = -INFINITY;
 #pragma unroll
       for (int i = 0; i < kSets; ++i) {
-        if (!kAll && i >= nb) continue;
+        if (!kAll && i >= nb) {
+          x.v[i][0] = x.v[i][1] = x.v[i][2] = x.v[i][3] = -INFINITY;
+          continue;
+        }
         uint32_t k0[kPack][W], k1[kPack][W], kp0[NG], kp1[NG];
 #pragma unroll
         for (int r = 0; r < kPack; ++r) {
@@ -586,48 +603,70 @@ __global__ void __launch_bounds__(32 * kWarps, kSmWarps / kWarps) kv4_decode_ker
             o[2 + c] = fmaf(m1, qs[n2][c], n2 ? o[2 + c] : -mx[c]);
           }
         }
-        // 2^23 + biased exponent of the largest scale of each token's V row (at least -40): added to x it
-        // rounds it to an integer, close enough for a bound
-        uint32_t vp0[NG], vp1[NG];
-        lds_words<NG>(vp0, rec + F::kVP + g * 4 * NG);
-        lds_words<NG>(vp1, rec + F::kVP + (g + 8) * 4 * NG);
-        uint32_t v0 = uint32_t(127 - 40) << 23, v1 = v0;
-#pragma unroll
-        for (int n2 = 0; n2 < NG; ++n2) {
-          v0 = max(v0, vp0[n2]);
-          v1 = max(v1, vp1[n2]);
-        }
-        const float e0 = __uint_as_float(0x4b000000u | v0 >> 23), e1 = __uint_as_float(0x4b000000u | v1 >> 23);
+        const float2 e = exponents(rec);
         const int valid = left - 16 * mine;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const float y = fmaf(alpha[c & 1], t[c], o[c]);
           x.v[i][c] = kAll || g + 8 * (c >> 1) < valid ? y : -INFINITY;
         }
-        top[0] = fmaxf(top[0], fmaxf(x.v[i][0] + e0, x.v[i][2] + e1));
-        top[1] = fmaxf(top[1], fmaxf(x.v[i][1] + e0, x.v[i][3] + e1));
+        top[0] = fmaxf(top[0], fmaxf(x.v[i][0] + e.x, x.v[i][2] + e.y));
+        top[1] = fmaxf(top[1], fmaxf(x.v[i][1] + e.x, x.v[i][3] + e.y));
+      }
+    };
+    // The exponent of the largest weight of each column of the warp, less where it is settled.
+    auto above = [&](float (&m)[2]) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        m[c] = fmaxf(m[c], __shfl_xor_sync(0xffffffff, m[c], 4));
+        m[c] = fmaxf(m[c], __shfl_xor_sync(0xffffffff, m[c], 8));
+        m[c] = fmaxf(m[c], __shfl_xor_sync(0xffffffff, m[c], 16));
+        m[c] -= 8388608.f + 127.f + kSettled;
       }
     };
     // Moves the reference where a weight would outgrow it: most pairs only learn that none does.
-    auto settle = [&](Scores& x, const float (&top)[2]) {
+    auto settle = [&](uint32_t recs, Scores& x, const float (&top)[2]) {
       if (__any_sync(0xffffffff, first || fmaxf(top[0], top[1]) > 8388608.f + 127.f + kLargest)) {
-        float fac[2];
+        float by[2] = {top[0], top[1]}, fac[2];
+        above(by);
+        bool far = false;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float m = top[c];
-          m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 4));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 8));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, 16));
-          m -= 8388608.f + 127.f + kSettled;
           // up by `by`, where that is positive; the first time to where it belongs (a floor keeps it finite)
-          const float by = fmaxf(m, first ? -1e30f : 0.f);
-          const float f = first ? 0.f : exp2_approx(-by);
-          mx[c] += by;
+          by[c] = fmaxf(by[c], first ? -1e30f : 0.f);
+          far |= fabsf(by[c]) > 4194304.f && fabsf(by[c]) < 1e29f;
 #pragma unroll
           for (int i = 0; i < kSets; ++i) {
-            x.v[i][c] -= by;
-            x.v[i][2 + c] -= by;
+            x.v[i][c] -= by[c];
+            x.v[i][2 + c] -= by[c];
           }
+        }
+        if (__any_sync(0xffffffff, far)) {
+          // Scores so large that x + exponent was rounded to more than a whole number: the rest of the way from
+          // what is left of them.  Without it scores of 2^29 and more can leave every weight zero or one infinite.
+          float rest[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < kSets; ++i) {
+            const float2 e = exponents(recs + (kPack == 2 ? half : i) * F::kRec);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) rest[c] = fmaxf(rest[c], fmaxf(x.v[i][c] + e.x, x.v[i][2 + c] + e.y));
+          }
+          above(rest);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float r = by[c] != 0.f && rest[c] > -1e29f ? rest[c] : 0.f;
+            by[c] += r;
+#pragma unroll
+            for (int i = 0; i < kSets; ++i) {
+              x.v[i][c] -= r;
+              x.v[i][2 + c] -= r;
+            }
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float f = first ? 0.f : exp2_approx(-by[c]);
+          mx[c] += by[c];
           l[c] *= f;
 #pragma unroll
           for (int n2 = 0; n2 < NG; ++n2) um[n2][c] *= f;
@@ -726,7 +765,7 @@ __global__ void __launch_bounds__(32 * kWarps, kSmWarps / kWarps) kv4_decode_ker
     for (int i = 0; i < whole_pairs; ++i) {
       const uint32_t now = arrived();
       scores(now, Whole<true>(), kNB, 0, x, top);
-      settle(x, top);
+      settle(now, x, top);
       weigh(now, Whole<true>(), kNB, 0, x);
       __syncwarp();  // every lane has read the slot
       issue();
@@ -737,7 +776,7 @@ __global__ void __launch_bounds__(32 * kWarps, kSmWarps / kWarps) kv4_decode_ker
       const int nb = min(kNB, re - u);
       const int left = min(head_len(p, bh) - (u - pre[bh]) * 16, 16 * nb);  // tokens of these records that count
       scores(now, Whole<false>(), nb, left, x, top);
-      settle(x, top);
+      settle(now, x, top);
       weigh(now, Whole<false>(), nb, left, x);
       __syncwarp();
       issue();
