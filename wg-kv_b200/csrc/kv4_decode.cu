@@ -56,6 +56,8 @@
 // 0.55 of the issue slots and 0.58 of the integer pipe.  A single sequence of 2K tokens takes 8.8 us, all of it
 // latency: four dependent look-ups (lengths, table, records; then the counter and the partial results) of 0.4 to 1
 // us each around one pair of records per warp.
+#include <algorithm>
+
 #include "kv4.cuh"
 #include "runtime.h"
 
@@ -966,16 +968,29 @@ size_t workspace_need(int64_t kv_heads, int group, int D, int sms) {
   return kCounterBytes + size_t(BH + sms * (kSmWarps / 4)) * G * (D + 4) * 4 + 256;
 }
 
+// What an SM has for its CTAs, each of which costs kCtaSmem more than it asks for.
+constexpr size_t kSmSmem = 228 * 1024, kCtaSmem = 1024;
+
 struct DecodeLaunch {
   Kv4DecodeParams p;
   cudaStream_t stream;
   int sms, status;
+  template <int D, int NG>
+  size_t smem_of(int warps) const {
+    return fixed_smem(warps, p.BH, p.G, D) + size_t(warps) * kSlots * kNB * Kv4<D, NG>::kRec;
+  }
+  // CTAs that are on an SM together.  Beside the ring and the merge rows, which let kSmWarps warps in, a CTA
+  // holds the line of all heads (8 bytes each), so that from 1800 to 5000 heads up, by D, group and G, three CTAs
+  // of 4 warps do not fit, later two of 6 neither.
+  template <int D, int NG>
+  int resident(int warps) const {
+    return int(std::min(size_t(kSmWarps / warps), kSmSmem / (smem_of<D, NG>(warps) + kCtaSmem)));
+  }
   template <int D, int NG, int kPack, int kWarps>
   void launch() {
-    constexpr int kCtas = kSmWarps / kWarps;
+    const int ctas = resident<D, NG>(kWarps);  // a segment for each, all in one wave
     const auto kernel = kv4_decode_kernel<D, NG, kPack, kWarps>;
-    // at most 128 KB, 8192 heads' places in the line among them, or 190 KB of 12 warps
-    const size_t smem = fixed_smem(kWarps, p.BH, p.G, D) + size_t(kWarps) * kSlots * kNB * Kv4<D, NG>::kRec;
+    const size_t smem = smem_of<D, NG>(kWarps);
     p.slots = kSlots;
     static bool attr_set[64] = {false};
     int dev = 0;
@@ -988,7 +1003,7 @@ struct DecodeLaunch {
       if (dev < 64) attr_set[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(sms * kCtas);
+    cfg.gridDim = dim3(sms * ctas);
     cfg.blockDim = dim3(32 * kWarps);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -1001,9 +1016,13 @@ struct DecodeLaunch {
   }
   template <int D, int NG, int kPack>
   void warps() {
-    if (p.BH >= kManyHeads) return launch<D, NG, kPack, 4>();
     if constexpr (kPack == 1)
       if (p.BH < kFewHeads) return launch<D, NG, kPack, 12>();
+    // the form for many heads, unless their line leaves fewer of its warps on an SM than of the other's (4096 heads
+    // of 200 tokens: 115 us with three CTAs of 4 warps asked for, of which two fit, 70 us with two of 6; 8 rows a
+    // head and groups of 32, where only two CTAs of 4 or one of 6 fit: 113 us with three asked for, 78 with two,
+    // 112 with one of 12; 8192 such heads of 100 tokens: 248 us with three, 204 with one of 6)
+    if (p.BH >= kManyHeads && 4 * resident<D, NG>(4) >= 6 * resident<D, NG>(6)) return launch<D, NG, kPack, 4>();
     launch<D, NG, kPack, 6>();
   }
   template <int D, int NG>
