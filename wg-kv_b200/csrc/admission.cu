@@ -502,7 +502,8 @@ struct PutRowKv4 {
   }
 };
 
-// Not inlined: five instances in kernels that are tuned for the bf16 pool.
+// Not inlined: five instances in kernels that are tuned for the bf16 pool.  A kernel that calls it has 64
+// registers at least.
 __device__ __noinline__ void put_row_kv4(uint8_t* kv4, int D, int group, int64_t row, const uint16_t* k,
                                          const uint16_t* v) {
   kv4_dispatch(D, group, PutRowKv4{kv4, row, k, v});
@@ -548,6 +549,7 @@ __device__ __forceinline__ void ring_position(const wgkv_pool& P, int& ins, int&
   }
 }
 
+template <bool kKv4>  // whether the pool is held in 4 bits (in one kernel for both, bf16 rows took 64 registers, not 32)
 __global__ void __launch_bounds__(256) decode_append_kernel(PoolArgs pa, int layer, int ins, int cur, RowSrc K,
                                                             RowSrc V, RowSrc PK, int32_t* cache_seqlens) {
   const wgkv_pool& P = pa.P;
@@ -558,7 +560,7 @@ __global__ void __launch_bounds__(256) decode_append_kernel(PoolArgs pa, int lay
   ring_position(P, ins, cur);
   const int b = i / Hk, h = i - b * Hk;
   const int64_t row = (int64_t(layer) * BH + i) * P.window + ins;
-  if (P.kv4) {
+  if constexpr (kKv4) {
     put_row_kv4(P.kv4, D, P.kv4_group, row, K.p + b * K.sb + h * K.sh, V.p + b * V.sb + h * V.sh);
   } else {
     copy_row<false>(P.k + row * D, K.p + b * K.sb + h * K.sh, D, lane, 32);
@@ -1139,8 +1141,8 @@ extern "C" int wgkv_decode_append(const wgkv_pool* pool, int layer, int insert_p
   PoolArgs pa{*pool};
   const int BH = pool->batch * pool->kv_heads;
   RowSrc K{k_new, k_sb, k_sh, 0}, V{v_new, v_sb, v_sh, 0}, PK{pre_k_new, pk_sb, pk_sh, 0};
-  decode_append_kernel<<<(BH + 7) / 8, 256, 0, as_stream(stream)>>>(pa, layer, insert_pos, cur_local_len, K, V, PK,
-                                                                    cache_seqlens);
+  const auto kernel = pool->kv4 ? decode_append_kernel<true> : decode_append_kernel<false>;
+  kernel<<<(BH + 7) / 8, 256, 0, as_stream(stream)>>>(pa, layer, insert_pos, cur_local_len, K, V, PK, cache_seqlens);
   return cudaGetLastError() == cudaSuccess ? WGKV_OK : WGKV_ECUDA;
 }
 
