@@ -44,3 +44,33 @@ def test_decode_most_heads(D, group, G, B, Hk, longest):
         assert (over <= 0).all(), f"sequence {b}: {(over > 0).sum()} outside, worst by {over.max():.3g}"
     empty = np.repeat(lens == 0, G, 1)
     assert not got[:, 0][empty].any() and got[:, 0][~empty].any(-1).all()
+
+
+@pytest.mark.parametrize("D,group,G,B,Hk,width,T", [(64, 64, 1, 512, 8, 511, 4096), (64, 32, 8, 1, 60, 34900, 4096)])
+def test_decode_most_records(D, group, G, B, Hk, width, T):
+    """Just under 2^29 records of 16 tokens, the most a call takes: whole heads of one page over and over, so
+    that every head's result is that of the page alone.
+
+    A lane adds the same few numbers once for every pair of records that its warp takes, so fp32 sums of n terms
+    are off by up to n 2^-24 of the terms' sizes, in the numerator and in the denominator."""
+    import wgkv
+    rng = np.random.default_rng(B)
+    records = B * Hk * width * T // 16
+    assert 0.99 * 2 ** 29 < records < 2 ** 29
+    cache = wgkv.kv4_alloc(1, T, D, group)
+    k, v = K4.bf16(0.1 * rng.standard_normal((1, 1, T, D))), K4.bf16(rng.standard_normal((1, 1, T, D)) + 2.0)
+    wgkv.kv4_append(dev(k), dev(v), cache, dev_i([[0]]), dev_i([[[0]]]))
+    q1 = K4.bf16(rng.standard_normal((1, 1, G, D)))
+    table = torch.zeros(B, Hk, width, dtype=torch.int32, device="cuda")
+    lens = torch.full((B, Hk), width * T, dtype=torch.int32, device="cuda")
+    q = dev(q1).expand(B, Hk, G, D).reshape(B, 1, Hk * G, D)
+    out = wgkv.paged_decode_kv4(q, cache, lens, table, D ** -0.5)
+    torch.cuda.synchronize()
+    wgkv.check_errors()
+    parts = K4.unpack(cache.cpu().numpy(), D, group)
+    want, tol = K4.decode(q1, [[tuple(parts[:3])]], [[tuple(parts[3:])]], np.array([[T]]), D ** -0.5)
+    pairs = width * T / 32 / 4  # of a head, over the fewest warps of a CTA
+    p_v = K4.values(parts[3], np.abs(parts[4]), parts[5]).max()
+    tol = tol + 2 * min(pairs, records / 2 / 148 / 6) * 2.0 ** -24 * p_v
+    got = out.double().cpu().numpy().reshape(-1, G, D)
+    assert (np.abs(got - want.reshape(1, G, D)) <= tol.reshape(1, G, D)).all(), np.abs(got - want.reshape(1, G, D)).max()

@@ -227,8 +227,9 @@ WGKV_DEV int head_len(const Kv4DecodeParams& p, int bh) {
   return min(max(__ldg(p.seqlens + (bh >> p.halves)), 0), p.c.width * p.c.page);
 }
 
-// ceil(n / d) for 0 <= n < 2^29, d > 0 and a quotient below 2^21 (n over the CTAs, or below their number):
-// in fp32 it is at most one off.
+// ceil(n / d) for 0 <= n < 2^29 + 2^20, d > 0 and a quotient below 2^22 (the line's records over 148 CTAs at
+// least, or a number of CTAs): __fdividef is off by up to 2 ulps, 1/2 at such quotients, and n by up to 32 in fp32,
+// less than 1/4 over the CTAs, so the fp32 quotient is at most one off.
 WGKV_DEV int ceil_div(int n, int d) {
   n += d - 1;
   int q = int(__fdividef(float(n), float(d)));
