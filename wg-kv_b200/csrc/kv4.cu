@@ -1,10 +1,10 @@
 // Writing rows into the 4-bit KV cache and reading them back (format: kv4.cuh).
 //
 // Both are one pass over the data and bound by HBM: a token costs 4 D bytes of bf16 and D + 8 D / group of
-// codes.  Measured on B200, D = 128, groups of 64, 64K rows of 8 heads (343 MB each way): writing 62 us,
-// 5.5 TB/s, 0.84 of the copy bandwidth with 0.77 of the issue slots busy (102 warp instructions a row,
-// 5 per value and lane: unpack, subtract, multiply-add, round down, shift in); reading 53
-// us, 6.5 TB/s, 0.99.
+// codes.  Measured on B200, D = 128, groups of 64, 64K rows of 8 heads (343 MB each way), in replayed graphs:
+// writing 62 us, 5.5 TB/s, 0.84 of the copy bandwidth (66 us by itself on cold data, with 0.77 of the issue slots
+// busy: 102 warp instructions a row, 5 per value and lane: unpack, subtract, multiply-add, round down, shift in);
+// reading 53 us, 6.5 TB/s, 0.99 (54 us by itself).
 #include <type_traits>
 #include <utility>
 

@@ -50,12 +50,20 @@
 // results fed by bulk copies into shared memory (25 against 21 us with 8 heads of 16 rows).  The copies alone,
 // without any arithmetic, take 85 us.
 //
-// Measured on B200: 3.5M tokens x KV heads (G = 4, D = 128, groups of 64, 504 MB) in 91 us, 5.5 TB/s, 0.85
-// of the copy bandwidth, 3 times as fast as the bf16 kernel on the same tokens (1.79 GB, 287 us).  What bounds it
-// there is latency with 3 warps per scheduler (168 registers): 230 instructions a record, 80 of them unpacking, at
-// 0.55 of the issue slots and 0.58 of the integer pipe.  A single sequence of 2K tokens takes 8.8 us, all of it
-// latency: four dependent look-ups (lengths, table, records; then the counter and the partial results) of 0.4 to 1
-// us each around one pair of records per warp.
+// Measured on B200: 3.5M tokens x KV heads (G = 4, D = 128, groups of 64, 504 MB) in 98 us by itself with nothing
+// of them in L2, 5.1 TB/s, 0.79 of the copy bandwidth, and 91 us a call in a replayed graph of 20 calls, whose set-up
+// overlaps the call before and finds a part of the data in L2; the bf16 kernel takes 287 us on the same tokens (1.79
+// GB).  The times by which variants are compared in this file are of such graphs.  What bounds it there is latency
+// with 3 warps per scheduler (168 registers): 223 instructions a record, 72 of them unpacking, at 0.51 of the issue
+// slots and 0.57 of the integer pipe.  A single sequence of 2K tokens takes 9.0 us, all of it latency: four dependent
+// look-ups (lengths, table, records; then the counter and the partial results) of 0.4 to 1 us each around one pair
+// of records per warp.
+//
+// The launch is a programmatic dependent one whatever pdl_enabled() says of the others: set-up overlaps the kernel
+// before, and the queries, lengths and tables are read behind griddep_wait().  It never cost (a step of a 4-bit
+// Llama-3.1-8B shape in graph replay 3.99 ms with, 4.00 without; Llama-3.2-1B 1.090 with, 1.100 without; append and
+// attention of 32 sequences 60.6 with, 61.3 us without).
+
 #include <algorithm>
 
 #include "kv4.cuh"
