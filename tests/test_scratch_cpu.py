@@ -48,7 +48,8 @@ def overlapping(monkeypatch, first_wait=0.5):
         return Block(n)
 
     stand_in = SimpleNamespace(
-        empty=allocate, zeros=allocate, uint8="uint8", int32="int32", device=torch.device, cuda=SimpleNamespace(
+        empty=allocate, zeros=allocate, uint8="uint8", int32="int32", device=torch.device,
+        inference_mode=torch.inference_mode, cuda=SimpleNamespace(
             is_current_stream_capturing=lambda: False, current_device=lambda: 0, Stream=lambda: Stream(1),
             stream=lambda s: contextlib.nullcontext(), device=lambda d: contextlib.nullcontext()))
     monkeypatch.setattr(runtime, "torch", stand_in)

@@ -39,11 +39,12 @@ def _new_error_word(index: int) -> torch.Tensor:
 
     It is made on a stream of its own and waited for: the current stream may have work queued behind which
     the zero would arrive after another stream's flag, or may be capturing a graph, in whose memory the word
-    would be set to zero by every replay."""
+    would be set to zero by every replay.  And it is an ordinary tensor, which check_errors() may reset in or
+    out of inference mode."""
     mode = lib.wgkv_thread_capture_mode(2)
     check(min(mode, 0), "wgkv_thread_capture_mode")
     try:
-        with torch.cuda.device(index):
+        with torch.cuda.device(index), torch.inference_mode(False):
             stream = torch.cuda.Stream()
             while lib.wgkv_stream_capture_id(stream.cuda_stream):  # torch deals its streams in turns
                 stream = torch.cuda.Stream()
