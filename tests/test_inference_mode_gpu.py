@@ -44,3 +44,31 @@ def run(script):
 
 def test_errors_of_calls_in_inference_mode_are_reported_and_reset():
     run(ERRORS)
+
+
+SCRATCH = """
+import torch
+import wgkv
+
+dev = "cuda"
+
+
+def attend(batch, kv_heads, group, d):
+    n = batch * kv_heads
+    lens = torch.full((batch, kv_heads), 20, dtype=torch.int32, device=dev)
+    table = torch.arange(2 * n, dtype=torch.int32, device=dev).view(batch, kv_heads, 2)
+    q = torch.randn(batch, 1, kv_heads * group, d, device=dev).bfloat16()
+    k = torch.randn(2 * n, 16, d, device=dev).bfloat16()
+    return wgkv.paged_decode(q, k, k, lens, table, 0.125)
+
+
+with torch.inference_mode():
+    attend(1, 2, 8, 128)  # few counters, long partial results
+attend(16, 8, 1, 64)      # more counters in the same scratch, which are set to zero first
+wgkv.check_errors()
+print("good")
+"""
+
+
+def test_scratch_made_in_inference_mode_serves_outside_of_it():
+    run(SCRATCH)

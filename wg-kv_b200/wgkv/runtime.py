@@ -89,7 +89,8 @@ def workspace(device, purpose: str, nbytes: int, zero_prefix: int = 0) -> torch.
     key = (d.index, torch.cuda.current_stream(d).cuda_stream, purpose)
     ent = _workspaces.get(key)
     if ent is None or ent[0].numel() < nbytes:
-        ws = torch.empty(max(nbytes, zero_prefix, 256), dtype=torch.uint8, device=d)
+        with torch.inference_mode(False):  # later calls may zero a longer prefix out of inference mode
+            ws = torch.empty(max(nbytes, zero_prefix, 256), dtype=torch.uint8, device=d)
         zeroed = 0
     else:
         ws, zeroed = ent
