@@ -535,7 +535,8 @@ WGKV_API int wgkv_kv4_append(const uint16_t* k, int64_t k_sb, int64_t k_sh, int6
 /*
  * Reads rows back: out_k / out_v (B, Hk, rows, D) bf16, contiguous and 16-byte aligned; row i of (b, h) is
  * scale * code + minimum, rounded to fp32 and then to bf16, of position start[b, h] + i (start NULL: 0) for
- * i < min(counts[b, h], rows), zero behind it.  Positions and page ids out of range read as zero and flag the same errors.
+ * i < min(counts[b, h], rows), zero behind it.  Positions and page ids out of range read as zero and flag the
+ * same errors.
  */
 WGKV_API int wgkv_kv4_read(const uint8_t* cache, int64_t num_pages, int page_size, int head_dim, int group,
                            const int32_t* start, const int32_t* counts, const int32_t* block_table,
@@ -551,7 +552,7 @@ WGKV_API int wgkv_kv4_read(const uint8_t* cache, int64_t num_pages, int page_siz
  * bits while they are within 2^-20 of a head's largest such weight (over all groups of its tokens), and by no
  * more than 2^-31 of that largest weight below.  So the tail behind a heavy token, or a group whose scales are
  * far below those of another group of the same rows, is held to full precision down to that distance.
- * A token whose scales are all below 2^-40 counts as one of 2^-40 there: values of V of 2^50 and more in rows
+ * A token whose scales are all below 2^-40 counts as one of 2^-40 there: values of V of 2^45 and more in rows
  * that are that flat may overflow.
  * Constraints: (head_dim, group) as above; page_size % 16 == 0; Hq % Hk == 0; Hq / Hk <= 16;
  * B * Hk <= 4096; B * Hk * table_width * page_size / 16 < 2^29 (2^28 if Hq / Hk > 8); 16-byte aligned q, out

@@ -100,3 +100,21 @@ def test_decode_on_forked_streams_of_one_graph(wgkv):
     wgkv.check_errors()
     assert all(torch.equal(x, w) for xs, w in zip(got, want) for x in xs)
     assert all(torch.equal(wgkv.paged_decode_kv4(q, cache, ln, tb, 0.125), w) for q, w in zip(qs, want))
+
+
+@pytest.mark.parametrize("D,group,G", [(128, 64, 4), (64, 64, 8)])
+def test_decode_large_constant_values(wgkv, D, group, G):
+    """Rows of V whose groups hold one value each (scale 0), up to the size that the documentation allows, next to
+    scores that grow with every token so that the reference keeps moving: sums of p times V stay finite, and the
+    output within the oracle's bound."""
+    rng = np.random.default_rng(D)
+    n = 1500
+    one = np.array([[n]], np.int32)
+    k = K4.bf16(0.1 * rng.standard_normal((1, 1, n, D)) + np.linspace(0, 2, n)[:, None])
+    v = K4.bf16(np.repeat(2.0 ** 44 * rng.choice([-1.0, 1.0], (1, 1, n, D // group)), group, -1))
+    cache, tbl, hk, hv = filled(wgkv, rng, one, D, group, 16, rows=(k, v))
+    q = K4.bf16(1.0 + 0.1 * rng.standard_normal((1, 1, G, D)))
+    out = wgkv.paged_decode_kv4(dev(q), cache, dev_i(one), dev_i(tbl), D ** -0.5)
+    wgkv.check_errors()
+    want, tol = K4.decode(q, hk, hv, one, D ** -0.5)
+    assert (np.abs(out.double().cpu().numpy() - want) <= tol).all()

@@ -155,8 +155,8 @@ WGKV_DEV uint32_t swz128(uint32_t row, uint32_t chunk) { return row * 128u + ((c
 WGKV_DEV void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 WGKV_DEV void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// Programmatic dependent launch through launch_pdl is opt-in (WGKV_PDL=1 in the environment; the decode attention over a
-// 4-bit cache always launches so, for the reasons given there): it won little at batch 1
+// Programmatic dependent launch through launch_pdl is opt-in (WGKV_PDL=1 in the environment; the decode
+// attention over a 4-bit cache always launches so, for the reasons given there): it won little at batch 1
 // on the Llama-3.2-1B decoder step and cost 13 % on the Llama-3.1-8B step (4.10 -> 4.70 ms), whose
 // projections run many waves.  Without it griddepcontrol is a no-op and the kernels run in stream order.
 inline bool pdl_enabled() {

@@ -1029,8 +1029,8 @@ struct DecodeLaunch {
       if (p.BH < kFewHeads) return launch<D, NG, kPack, 12>();
     // the form for many heads, unless their line leaves fewer of its warps on an SM than of the other's (4096 heads
     // of 200 tokens: 115 us with three CTAs of 4 warps asked for, of which two fit, 70 us with two of 6; 8 rows a
-    // head of 100 tokens, groups of 32, where only two CTAs of 4 or one of 6 fit: 113 us with three asked for, 78 with two,
-    // 112 with one of 12; 8192 such heads of 100 tokens: 248 us with three, 204 with one of 6)
+    // head of 100 tokens, groups of 32, where only two CTAs of 4 or one of 6 fit: 113 us with three asked for, 78
+    // with two, 112 with one of 12; 8192 such heads of 100 tokens: 248 us with three, 204 with one of 6)
     if (p.BH >= kManyHeads && 4 * resident<D, NG>(4) >= 6 * resident<D, NG>(6)) return launch<D, NG, kPack, 4>();
     launch<D, NG, kPack, 6>();
   }
